@@ -99,8 +99,9 @@ def _quantise(x, fmt):
         y = x / scale
         ulp = torch.ldexp(torch.ones_like(y), torch.frexp(y)[1].clamp(min=-5) - 4)    # 4 bits of significand, least exponent -6
         return torch.round(y / ulp) * ulp, scale.squeeze(-1)
-    scale = (top / 127.0).clamp(min=2.0 ** -126)
-    inverse = (127.0 / top).clamp(max=2.0 ** 126)
+    most = torch.full_like(top, 127.0)   # (a tensor: torch divides by a number, and a number by a tensor, through a rounded reciprocal)
+    scale = (top / most).clamp(min=2.0 ** -126)
+    inverse = (most / top).clamp(max=2.0 ** 126)
     return torch.round(x * inverse), scale.squeeze(-1)
 
 
