@@ -1,0 +1,182 @@
+"""Decode attention of a batch behind a shared prefix on the GPU, 16-bit and 8-bit caches, against 64-bit references."""
+import math
+
+import pytest
+import torch
+
+from kvq_util import CODES, DTYPES, SCALE, check_attention, laid, random_cache
+from topk_attn_amd import ops
+from util import announce
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [(d, f) for d in DTYPES for f in ("16bit", "e4m3", "int8")]
+
+
+def _i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _source(gen, shape, dtype, fmt, layout):
+    """What PrefixDecodePlan takes for [B,N,H,128] rows, and the rows in 64 bits."""
+    if fmt == "16bit":
+        k, v = ((torch.randn(shape, generator=gen) * torch.exp(0.5 * torch.randn(shape[:-1] + (1,), generator=gen))).to(DTYPES[dtype]) for _ in range(2))
+        return (laid(k, layout), laid(v, layout)), k.double(), v.double()
+    held = [random_cache(gen, shape, fmt) for _ in range(2)]
+    cache = ops.QuantCache(laid(held[0][0], layout), laid(held[1][0], layout), laid(held[0][1], "heads"), laid(held[1][1], "heads"))
+    return cache, *(c.float().double() * s.double()[..., None] for c, s in held)
+
+
+def _as_prefix(source):
+    """[1,P,H,128] as the shared [P,H,128] form."""
+    if isinstance(source, tuple):
+        return source[0][0], source[1][0]
+    return ops.QuantCache(source.k_codes[0], source.v_codes[0], source.k_scale[0], source.v_scale[0])
+
+
+def _check(out, lse, q, pre, suf, length, G, dtype, fmt):
+    B, H = q.shape[0], q.shape[1] // G
+    none = torch.zeros((0, 128), dtype=torch.float64)
+    for b in range(B):
+        for h in range(H):
+            n = min(max(length[b], 0), suf[0].shape[1]) if suf else 0
+            k, v = (torch.cat([pre[i][0, :, h] if pre else none, suf[i][b, :n, h] if suf else none]) for i in range(2))
+            qs = slice(h * G, (h + 1) * G)
+            check_attention(out[b, qs], None if lse is None else lse[b, qs], q[b, qs], k, v, out.dtype, fmt != "16bit" or dtype == "f16")
+
+
+@pytest.mark.parametrize("dtype,fmt", KINDS)
+@pytest.mark.parametrize("B,H,G,P,S,layout", [(1, 1, 1, 1, 1, "tokens"), (2, 2, 4, 31, 5, "heads"), (5, 1, 4, 200, 33, "gaps"),
+                                              (9, 2, 2, 257, 40, "tokens"), (6, 1, 8, 1000, 130, "heads"), (17, 1, 4, 129, 3, "tokens"),
+                                              (33, 1, 8, 160, 2, "heads")])
+def test_prefix(dtype, fmt, B, H, G, P, S, layout):
+    announce("prefix %s %s B%d H%d G%d P%d S%d %s" % (dtype, fmt, B, H, G, P, S, layout))
+    gen = torch.Generator().manual_seed(B * P)
+    pre, kp, vp = _source(gen, (1, P, H, 128), dtype, fmt, layout)
+    suf, ks, vs = _source(gen, (B, S, H, 128), dtype, fmt, layout)
+    q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype])
+    length = [(S, 0, 1, S // 2, S + 3)[b % 5] for b in range(B)]
+    out, lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), suf, SCALE, G, suffix_len=_i32(length), return_lse=True)
+    _check(out, lse, q, (kp, vp), (ks, vs), length, G, dtype, fmt)
+    if B <= 6:
+        for splits in (1, 3):
+            out, lse = ops.prefix_decode(q.cuda(), pre, suf, SCALE, G, suffix_len=_i32(length), num_splits=splits, return_lse=True)
+            _check(out, lse, q, (kp, vp), (ks, vs), length, G, dtype, fmt)
+
+
+@pytest.mark.parametrize("dtype,fmt", KINDS)
+def test_prefix_alone_and_suffix_alone(dtype, fmt):
+    B, H, G = 4, 2, 2
+    gen = torch.Generator().manual_seed(2)
+    pre, kp, vp = _source(gen, (1, 100, H, 128), dtype, fmt, "tokens")
+    suf, ks, vs = _source(gen, (B, 50, H, 128), dtype, fmt, "heads")
+    q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype])
+    length = [50, 0, 1, 32]
+    announce("prefix alone %s %s" % (dtype, fmt))
+    out, lse = ops.prefix_decode(q.cuda(), pre, None, SCALE, G, return_lse=True)
+    _check(out, lse, q, (kp, vp), None, length, G, dtype, fmt)
+    out, lse = ops.prefix_decode(q.cuda(), None, suf, SCALE, G, suffix_len=_i32(length), return_lse=True)
+    _check(out, lse, q, None, (ks, vs), length, G, dtype, fmt)
+    out = ops.prefix_decode(q.cuda(), None, suf, SCALE, G)
+    _check(out, None, q, None, (ks, vs), [50] * B, G, dtype, fmt)
+
+
+@pytest.mark.parametrize("dtype,fmt", KINDS)
+def test_masked_places_hold_anything(dtype, fmt):
+    """NaN and infinities in the rows behind a suffix's length change nothing."""
+    B, H, G = 3, 2, 4
+    gen = torch.Generator().manual_seed(7)
+    pre, _, _ = _source(gen, (1, 90, H, 128), dtype, fmt, "tokens")
+    suf, _, _ = _source(gen, (B, 70, H, 128), dtype, fmt, "heads")
+    q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype]).cuda()
+    length = [70, 0, 37]
+    announce("prefix masked %s %s" % (dtype, fmt))
+    clean = ops.prefix_decode(q, pre, suf, SCALE, G, suffix_len=_i32(length))
+    for b in range(B):
+        for t in (suf if fmt == "16bit" else (suf.k_scale, suf.v_scale)):
+            t[b, length[b]:] = math.nan if b == 2 else math.inf
+    assert torch.equal(clean, ops.prefix_decode(q, pre, suf, SCALE, G, suffix_len=_i32(length)))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_extreme_16bit_rows(dtype):
+    """Logits of -infinity for every key but one, and the largest values of the type."""
+    B, H, G, P = 2, 1, 2, 64
+    dt = DTYPES[dtype]
+    k = torch.zeros((1, P, H, 128), dtype=dt)
+    v = torch.full((1, P, H, 128), torch.finfo(dt).max, dtype=dt)
+    q = torch.ones((B, H * G, 128), dtype=dt)
+    k[0, :, 0, 0] = -math.inf
+    k[0, 41] = 1.0
+    v[0, 41] = -2.0
+    announce("prefix extremes %s" % dtype)
+    out, lse = ops.prefix_decode(q.cuda(), (k.cuda(), v.cuda()), None, SCALE, G, return_lse=True)
+    assert (out == -2.0).all() and torch.allclose(lse.cpu(), torch.full((B, 2), 128 * SCALE), rtol=1e-6)
+    k[0, 41] = -math.inf                    # nothing but -infinity: no weight anywhere, like a row without keys
+    out, lse = ops.prefix_decode(q.cuda(), (k.cuda(), v.cuda()), None, SCALE, G, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    k.zero_()                               # equal weights over the largest numbers: their mean
+    v.fill_(torch.finfo(dt).max)
+    out = ops.prefix_decode(q.cuda(), (k.cuda(), v.cuda()), None, SCALE, G)
+    assert (out == torch.finfo(dt).max).all()
+
+
+def test_equals_attention_over_the_whole():
+    """Prefix and suffix of an 8-bit cache against the decode over one cache that holds both, within both bounds."""
+    B, H, G, P, S = 3, 2, 4, 500, 60
+    gen = torch.Generator().manual_seed(17)
+    pre, kp, vp = _source(gen, (1, P, H, 128), "bf16", "int8", "heads")
+    suf, ks, vs = _source(gen, (B, S, H, 128), "bf16", "int8", "heads")
+    q = torch.randn((B, H * G, 128), generator=gen).bfloat16()
+    whole = ops.QuantCache(*(torch.cat([getattr(pre, n).expand(B, *getattr(pre, n).shape[1:]), getattr(suf, n)], 1).contiguous()
+                             for n in ("k_codes", "v_codes", "k_scale", "v_scale")))
+    length = [60, 0, 31]
+    announce("prefix and whole")
+    a = ops.prefix_decode(q.cuda(), pre, suf, SCALE, G, suffix_len=_i32(length), return_lse=True)
+    b = ops.kvq_flash_decode(q.cuda(), whole, SCALE, G, kv_len=_i32([P + n for n in length]), return_lse=True)
+    for out, lse in (a, b):
+        _check(out, lse, q, (kp, vp), (ks, vs), length, G, "bf16", "int8")
+
+
+@pytest.mark.parametrize("fmt", ["16bit", "int8"])
+def test_graph_replays(fmt):
+    """Two captured graphs and eager calls in turn: every replay gives what an eager call gives."""
+    B, H, G = 5, 2, 4
+    gen = torch.Generator().manual_seed(23)
+    pre, _, _ = _source(gen, (1, 2000, H, 128), "bf16", fmt, "tokens")
+    suf, _, _ = _source(gen, (B, 100, H, 128), "bf16", fmt, "heads")
+    length = _i32([100, 0, 50, 1, 99])
+    qs = [torch.randn((B, H * G, 128), generator=gen).bfloat16().cuda() for _ in range(2)]
+    plans = [ops.PrefixDecodePlan(q, pre, suf, SCALE, G, suffix_len=length, return_lse=True) for q in qs]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    announce("prefix graphs %s" % fmt)
+    torch.cuda.synchronize()
+    for g, p in zip(graphs, plans):
+        with torch.cuda.graph(g):
+            p.run()
+    for step in range(4):
+        for q in qs:
+            q.copy_(torch.randn(q.shape, generator=gen))
+        for g in graphs:
+            g.replay()
+        want = [ops.prefix_decode(q, pre, suf, SCALE, G, suffix_len=length, return_lse=True) for q in qs]
+        torch.cuda.synchronize()
+        for p, (out, lse) in zip(plans, want):
+            assert torch.equal(p.out, out) and torch.equal(p.lse, lse)
+        length.sub_(1).clamp_(min=0)
+
+
+def test_offsets_beyond_32_bits():
+    """A prefix whose last rows lie beyond 4 GiB."""
+    P, stride = 300, 1 << 23
+    gen = torch.Generator().manual_seed(8)
+    k, v = (torch.randn((1, P, 1, 128), generator=gen).half() for _ in range(2))
+    far = []
+    for x in (k, v):
+        t = torch.zeros((P * stride,), dtype=torch.float16, device="cuda").as_strided((P, 1, 128), (stride, 128, 1))
+        t.copy_(x[0])
+        far.append(t)
+    q = torch.randn((2, 4, 128), generator=gen).half()
+    announce("prefix far offsets")
+    out, lse = ops.prefix_decode(q.cuda(), tuple(far), None, SCALE, 4, return_lse=True)
+    _check(out, lse, q, (k.double(), v.double()), None, [0, 0], 4, "f16", "16bit")

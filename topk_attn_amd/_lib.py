@@ -1,4 +1,5 @@
-"""ctypes binding of libtka.so: the structs and prototypes of include/topk_attn.h, field for field."""
+"""ctypes binding of libtka.so: the structs and prototypes of include/topk_attn.h and include/topk_attn_kvq.h, field for
+field."""
 import ctypes as C
 import os
 
@@ -130,6 +131,56 @@ for _v in RA_VARIANTS:
     for _k in RA_TOPKS:
         PROTOTYPES["launch_retrieval_attention%s_%d" % (_v, _k)] = (None, [_p, _p, _p, _p, C.c_int])
 
+
+# ---- include/topk_attn_kvq.h: 8-bit K/V caches and shared prefixes ----
+
+TKA_KV_16BIT, TKA_KV_E4M3, TKA_KV_INT8 = 0, 1, 2
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("format", _i32), ("batch", _i32),
+                ("num_kv_heads", _i32), ("head_dim", _i32), ("rows", _i64), ("stride_b", _i64), ("stride_n", _i64),
+                ("stride_h", _i64), ("scale_stride_b", _i64), ("scale_stride_n", _i64), ("scale_stride_h", _i64)]
+
+
+class KvqWriteArgs(C.Structure):
+    _fields_ = [("cache", KvCache), ("k", _p), ("v", _p), ("dtype", _i32), ("num_tokens", _i32), ("stride_b", _i64),
+                ("stride_n", _i64), ("stride_h", _i64), ("start", _p), ("count", _p), ("stream", _p)]
+
+
+class KvqReadArgs(C.Structure):
+    _fields_ = KvqWriteArgs._fields_
+
+
+class KvqScoresArgs(C.Structure):
+    _fields_ = [("cache", KvCache), ("q", _p), ("dtype", _i32), ("group", _i32), ("q_stride_b", _i64), ("kv_len", _p),
+                ("scale", _f), ("reserved0", _i32), ("out_scores", _p), ("stream", _p)]
+
+
+class KvqFlashDecodeArgs(C.Structure):
+    _fields_ = [("cache", KvCache), ("q", _p), ("out", _p), ("dtype", _i32), ("out_dtype", _i32), ("group", _i32),
+                ("num_splits", _i32), ("q_stride_b", _i64), ("out_stride_b", _i64), ("kv_len", _p), ("kv_idx", _p),
+                ("kv_count", _p), ("idx_len", _i32), ("scale", _f), ("out_lse", _p), ("workspace", _p),
+                ("workspace_bytes", _sz), ("stream", _p)]
+
+
+class PrefixDecodeArgs(C.Structure):
+    _fields_ = [("prefix", KvCache), ("suffix", KvCache), ("q", _p), ("out", _p), ("dtype", _i32), ("out_dtype", _i32),
+                ("group", _i32), ("num_splits", _i32), ("q_stride_b", _i64), ("out_stride_b", _i64), ("suffix_len", _p),
+                ("scale", _f), ("reserved0", _i32), ("out_lse", _p), ("workspace", _p), ("workspace_bytes", _sz),
+                ("stream", _p)]
+
+
+KVQ_PROTOTYPES = {
+    "tka_kvq_write": (C.c_int, [C.POINTER(KvqWriteArgs)]),
+    "tka_kvq_read": (C.c_int, [C.POINTER(KvqReadArgs)]),
+    "tka_kvq_scores": (C.c_int, [C.POINTER(KvqScoresArgs)]),
+    "tka_kvq_flash_decode_workspace_bytes": (_sz, [C.POINTER(KvqFlashDecodeArgs)]),
+    "tka_kvq_flash_decode": (C.c_int, [C.POINTER(KvqFlashDecodeArgs)]),
+    "tka_prefix_decode_workspace_bytes": (_sz, [C.POINTER(PrefixDecodeArgs)]),
+    "tka_prefix_decode": (C.c_int, [C.POINTER(PrefixDecodeArgs)]),
+}
+
 _lib = None
 
 
@@ -150,7 +201,7 @@ def lib():
         except ImportError:
             pass
         L = C.CDLL(LIB_PATH)
-        for name, (res, args) in PROTOTYPES.items():
+        for name, (res, args) in list(PROTOTYPES.items()) + list(KVQ_PROTOTYPES.items()):
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

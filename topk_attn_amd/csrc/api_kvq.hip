@@ -1,0 +1,330 @@
+// C ABI of the 8-bit K/V cache and of the shared-prefix attention (topk_attn_kvq.h): argument checks (before any HIP
+// call), split plans, workspace layout, launches.
+#include <string.h>
+
+#include <algorithm>
+#include <utility>
+
+#include "kvq.hpp"
+
+namespace tka {
+
+namespace {
+
+bool dtype_ok(int d) { return d == TKA_F16 || d == TKA_BF16; }
+bool group_ok(int g) { return g == 1 || g == 2 || g == 4 || g == 8; }
+bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+constexpr int64_t kMaxExtent = 1ll << 46;      // elements that a stride may span: more than any memory, and no sum of offsets passes 64 bits
+constexpr int64_t kMaxItems = 0x7fffffff;      // workgroups of a launch, partials of a call
+
+bool spans_ok(int64_t count, int64_t stride) { return stride >= 0 && (count <= 1 ? stride <= kMaxExtent : stride <= kMaxExtent / (count - 1)); }
+bool strides_ok(int64_t nb, int64_t nn, int64_t nh, int64_t b, int64_t n, int64_t h) { return spans_ok(nb, b) && spans_ok(nn, n) && spans_ok(nh, h); }
+
+// Rows of `width` at b*stride_b + t*stride_n + h*stride_h are disjoint when the strides nest.
+bool disjoint(int64_t width, int64_t nb, int64_t nn, int64_t nh, int64_t sb, int64_t sn, int64_t sh) {
+  std::pair<int64_t, int64_t> dims[3] = {{sb, nb}, {sn, nn}, {sh, nh}};
+  std::sort(dims, dims + 3);
+  int64_t extent = width;
+  for (const auto& d : dims) {
+    if (d.second <= 1) continue;
+    if (d.first < extent) return false;
+    extent += (d.second - 1) * d.first;
+  }
+  return true;
+}
+
+// A cache: sizes, format, strides, alignment.  `values`: its values are read or written too.
+int check_cache(const tka_kv_cache& c, bool values, bool allow_16bit) {
+  if (c.format != TKA_KV_E4M3 && c.format != TKA_KV_INT8 && !(allow_16bit && c.format == TKA_KV_16BIT)) return TKA_EUNSUPPORTED;
+  if (c.head_dim != TKA_HEAD_DIM) return TKA_EUNSUPPORTED;
+  if (c.batch < 1 || c.num_kv_heads < 1 || c.rows < 1) return TKA_EINVAL;
+  if (c.batch > 65535 || c.num_kv_heads > 65535 || c.rows > 0x7fffffffLL) return TKA_EUNSUPPORTED;
+  if (!c.k || (values && !c.v)) return TKA_EINVAL;
+  if (!strides_ok(c.batch, c.rows, c.num_kv_heads, c.stride_b, c.stride_n, c.stride_h)) return TKA_EINVAL;
+  if (c.rows > 1 && c.stride_n < TKA_HEAD_DIM) return TKA_EINVAL;
+  const int64_t per16 = c.format == TKA_KV_16BIT ? 8 : 16;   // elements of sixteen bytes
+  if ((c.stride_b | c.stride_n | c.stride_h) & (per16 - 1)) return TKA_EINVAL;
+  if (!aligned(c.k, 16) || (values && !aligned(c.v, 16))) return TKA_EINVAL;
+  if (c.format != TKA_KV_16BIT) {
+    if (!c.k_scale || (values && !c.v_scale)) return TKA_EINVAL;
+    if (!aligned(c.k_scale, 4) || (values && !aligned(c.v_scale, 4))) return TKA_EINVAL;
+    if (!strides_ok(c.batch, c.rows, c.num_kv_heads, c.scale_stride_b, c.scale_stride_n, c.scale_stride_h)) return TKA_EINVAL;
+  }
+  return TKA_OK;
+}
+
+KvRows rows_of(const tka_kv_cache& c) {
+  const int64_t width = c.format == TKA_KV_16BIT ? 2 : 1;
+  KvRows r;
+  r.k = (const unsigned char*)c.k;
+  r.v = (const unsigned char*)c.v;
+  r.ks = c.k_scale;
+  r.vs = c.v_scale;
+  r.stride_b = c.stride_b * width;
+  r.stride_n = c.stride_n * width;
+  r.stride_h = c.stride_h * width;
+  r.scale_b = c.scale_stride_b;
+  r.scale_n = c.scale_stride_n;
+  r.scale_h = c.scale_stride_h;
+  r.rows = c.rows;
+  return r;
+}
+
+// tka_kvq_write_args and tka_kvq_read_args have the same fields.
+template <typename Args>
+int check_copy(const Args* a, bool write) {
+  if (!a) return TKA_EINVAL;
+  const tka_kv_cache& c = a->cache;
+  const int rc = check_cache(c, true, false);
+  if (rc != TKA_OK) return rc;
+  if (!a->k || !a->v || a->num_tokens < 1) return TKA_EINVAL;
+  if (!dtype_ok(a->dtype)) return TKA_EUNSUPPORTED;
+  if (!strides_ok(c.batch, a->num_tokens, c.num_kv_heads, a->stride_b, a->stride_n, a->stride_h)) return TKA_EINVAL;
+  if ((a->stride_b | a->stride_n | a->stride_h) & 7) return TKA_EINVAL;
+  if (!aligned(a->k, 16) || !aligned(a->v, 16)) return TKA_EINVAL;
+  if ((int64_t)c.batch * c.num_kv_heads * a->num_tokens > kMaxItems) return TKA_EUNSUPPORTED;
+  if (write) {
+    if (!disjoint(TKA_HEAD_DIM, c.batch, c.rows, c.num_kv_heads, c.stride_b, c.stride_n, c.stride_h) ||
+        !disjoint(1, c.batch, c.rows, c.num_kv_heads, c.scale_stride_b, c.scale_stride_n, c.scale_stride_h))
+      return TKA_EINVAL;
+  } else if (!disjoint(TKA_HEAD_DIM, c.batch, a->num_tokens, c.num_kv_heads, a->stride_b, a->stride_n, a->stride_h)) {
+    return TKA_EINVAL;
+  }
+  return TKA_OK;
+}
+
+template <typename Args>
+KvqCopyParams copy_params(const Args* a) {
+  KvqCopyParams p;
+  p.cache = rows_of(a->cache);
+  p.k = (unsigned char*)const_cast<void*>((const void*)a->k);
+  p.v = (unsigned char*)const_cast<void*>((const void*)a->v);
+  p.stride_b = 2 * a->stride_b;
+  p.stride_n = 2 * a->stride_n;
+  p.stride_h = 2 * a->stride_h;
+  p.start = a->start;
+  p.count = a->count;
+  p.batch = a->cache.batch;
+  p.num_kv_heads = a->cache.num_kv_heads;
+  p.num_tokens = a->num_tokens;
+  p.tile_log2 = 0;
+  return p;
+}
+
+int check_query(const void* q, int dtype, int group, int64_t q_stride_b, int batch, int heads) {
+  if (!q) return TKA_EINVAL;
+  if (!dtype_ok(dtype) || !group_ok(group)) return TKA_EUNSUPPORTED;
+  const int64_t width = (int64_t)heads * group * TKA_HEAD_DIM;
+  if (!spans_ok(batch, q_stride_b) || (q_stride_b & 7) || !aligned(q, 16)) return TKA_EINVAL;
+  if (batch > 1 && q_stride_b < width) return TKA_EINVAL;
+  if ((int64_t)batch * heads * group > kMaxItems) return TKA_EUNSUPPORTED;
+  return TKA_OK;
+}
+
+int check_out(const void* out, int out_dtype, int64_t out_stride_b, int batch, int heads, int group) {
+  if (!out) return TKA_EINVAL;
+  if (!dtype_ok(out_dtype)) return TKA_EUNSUPPORTED;
+  if (!spans_ok(batch, out_stride_b) || (out_stride_b & 7) || !aligned(out, 16)) return TKA_EINVAL;
+  if (batch > 1 && out_stride_b < (int64_t)heads * group * TKA_HEAD_DIM) return TKA_EINVAL;
+  return TKA_OK;
+}
+
+int check_scores(const tka_kvq_scores_args* a) {
+  if (!a) return TKA_EINVAL;
+  int rc = check_cache(a->cache, false, false);
+  if (rc != TKA_OK) return rc;
+  rc = check_query(a->q, a->dtype, a->group, a->q_stride_b, a->cache.batch, a->cache.num_kv_heads);
+  if (rc != TKA_OK) return rc;
+  if (!a->out_scores || a->reserved0 != 0) return TKA_EINVAL;
+  if ((int64_t)a->cache.batch * a->cache.num_kv_heads * ((a->cache.rows + 255) / 256) > kMaxItems) return TKA_EUNSUPPORTED;
+  return TKA_OK;
+}
+
+// `len` positions in `want` splits of a multiple of kTps positions, `most` splits at most.
+constexpr int64_t kTps = 4 * kAttendTile;   // every wave of a workgroup has a tile
+void cut(int64_t len, int64_t want, int64_t most, int* splits, int* tps) {
+  want = std::min(std::max<int64_t>(want, 1), most);
+  int64_t per = (len + want - 1) / want;
+  per = (per + kTps - 1) / kTps * kTps;
+  *splits = (int)((len + per - 1) / per);
+  *tps = (int)per;
+}
+
+int log2_of(int group) { return group == 8 ? 3 : group >> 1; }
+
+struct Plan {
+  int row_tiles, row_blocks;
+  int shared_splits, shared_tps, own_splits, own_tps;
+};
+
+Plan plan_decode(const tka_kvq_flash_decode_args* a) {
+  Plan p = {1, 0, 0, 0, 0, 0};
+  const int64_t segs = (int64_t)a->cache.batch * a->cache.num_kv_heads;
+  const int64_t len = a->kv_idx ? a->idx_len : a->cache.rows;
+  cut(len, a->num_splits ? a->num_splits : 1024 / segs, TKA_MAX_SPLITS, &p.own_splits, &p.own_tps);
+  return p;
+}
+
+Plan plan_prefix(const tka_prefix_decode_args* a) {
+  Plan p = {1, 0, 0, 0, 0, 0};
+  const int64_t heads = a->prefix.num_kv_heads, batch = a->suffix.batch, query_rows = batch * a->group;
+  if (a->prefix.rows) {
+    p.row_tiles = query_rows <= 16 ? 1 : (query_rows <= 32 ? 2 : 4);
+    p.row_blocks = (int)((query_rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+    cut(a->prefix.rows, a->num_splits ? a->num_splits : 1024 / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
+  }
+  if (a->suffix.rows) cut(a->suffix.rows, 1024 / (heads * batch), TKA_MAX_SPLITS / 2, &p.own_splits, &p.own_tps);
+  return p;
+}
+
+int partials_ok(int64_t rows, const Plan& p) { return rows * (p.shared_splits + p.own_splits) <= kMaxItems ? TKA_OK : TKA_EUNSUPPORTED; }
+
+int check_decode(const tka_kvq_flash_decode_args* a) {
+  if (!a) return TKA_EINVAL;
+  const tka_kv_cache& c = a->cache;
+  int rc = check_cache(c, true, false);
+  if (rc != TKA_OK) return rc;
+  rc = check_query(a->q, a->dtype, a->group, a->q_stride_b, c.batch, c.num_kv_heads);
+  if (rc != TKA_OK) return rc;
+  rc = check_out(a->out, a->out_dtype, a->out_stride_b, c.batch, c.num_kv_heads, a->group);
+  if (rc != TKA_OK) return rc;
+  if (a->num_splits < 0 || a->num_splits > TKA_MAX_SPLITS) return TKA_EINVAL;
+  if (a->kv_idx ? a->idx_len < 1 : (a->kv_count != nullptr || a->idx_len != 0)) return TKA_EINVAL;
+  return partials_ok((int64_t)c.batch * c.num_kv_heads * a->group, plan_decode(a));
+}
+
+int check_prefix(const tka_prefix_decode_args* a) {
+  if (!a) return TKA_EINVAL;
+  tka_kv_cache pre = a->prefix, suf = a->suffix;
+  if (pre.format != suf.format || pre.num_kv_heads != suf.num_kv_heads || pre.batch != 1) return TKA_EINVAL;
+  if (pre.rows < 0 || suf.rows < 0 || a->reserved0 != 0) return TKA_EINVAL;
+  if (pre.rows + suf.rows == 0) return TKA_EINVAL;
+  int rc;
+  if (pre.rows && (rc = check_cache(pre, true, true)) != TKA_OK) return rc;
+  if (suf.rows && (rc = check_cache(suf, true, true)) != TKA_OK) return rc;
+  if (suf.batch < 1) return TKA_EINVAL;
+  if (suf.batch > 65535) return TKA_EUNSUPPORTED;
+  rc = check_query(a->q, a->dtype, a->group, a->q_stride_b, suf.batch, suf.num_kv_heads);
+  if (rc != TKA_OK) return rc;
+  rc = check_out(a->out, a->out_dtype, a->out_stride_b, suf.batch, suf.num_kv_heads, a->group);
+  if (rc != TKA_OK) return rc;
+  if (a->num_splits < 0 || a->num_splits > TKA_MAX_SPLITS / 2) return TKA_EINVAL;
+  return partials_ok((int64_t)suf.batch * suf.num_kv_heads * a->group, plan_prefix(a));
+}
+
+size_t partial_bytes(int64_t rows, const Plan& p) {
+  const size_t parts = (size_t)rows * (size_t)(p.shared_splits + p.own_splits);
+  return 2 * align_up(parts * sizeof(float), 256) + align_up(parts * TKA_HEAD_DIM * sizeof(float), 256);
+}
+
+// The workspace holds the partials: maxima, sums, accumulators.
+int run_attend(KvAttendParams p, const Plan& plan, int dtype, int format, void* workspace, hipStream_t stream) {
+  p.row_blocks = plan.row_blocks;
+  p.shared_splits = plan.shared_splits;
+  p.shared_tps = plan.shared_tps;
+  p.own_splits = plan.own_splits;
+  p.own_tps = plan.own_tps;
+  p.num_splits = plan.shared_splits + plan.own_splits;
+  const size_t parts = (size_t)p.batch * p.num_kv_heads * ((size_t)p.num_splits << p.group_log2);
+  unsigned char* ws = (unsigned char*)workspace;
+  p.part_m = (float*)ws;
+  p.part_l = (float*)(ws + align_up(parts * sizeof(float), 256));
+  p.part_acc = (float*)(ws + 2 * align_up(parts * sizeof(float), 256));
+  const int rc = launch_kv_attend(p, dtype, format, plan.row_tiles, stream);
+  if (rc != TKA_OK || p.num_splits == 1) return rc;
+  return launch_kv_combine(p, stream);
+}
+
+}  // namespace
+}  // namespace tka
+
+using namespace tka;
+
+extern "C" {
+
+int tka_kvq_write(const tka_kvq_write_args* a) {
+  const int rc = check_copy(a, true);
+  if (rc != TKA_OK) return rc;
+  return launch_kvq_write(copy_params(a), a->dtype, a->cache.format, (hipStream_t)a->stream);
+}
+
+int tka_kvq_read(const tka_kvq_read_args* a) {
+  const int rc = check_copy(a, false);
+  if (rc != TKA_OK) return rc;
+  return launch_kvq_read(copy_params(a), a->dtype, a->cache.format, (hipStream_t)a->stream);
+}
+
+int tka_kvq_scores(const tka_kvq_scores_args* a) {
+  const int rc = check_scores(a);
+  if (rc != TKA_OK) return rc;
+  KvqScoresParams p;
+  p.cache = rows_of(a->cache);
+  p.q = a->q;
+  p.q_stride_b = a->q_stride_b;
+  p.kv_len = a->kv_len;
+  p.scores = a->out_scores;
+  p.batch = a->cache.batch;
+  p.num_kv_heads = a->cache.num_kv_heads;
+  p.group = a->group;
+  p.scale = a->scale;
+  return launch_kvq_scores(p, a->dtype, a->cache.format, (hipStream_t)a->stream);
+}
+
+size_t tka_kvq_flash_decode_workspace_bytes(const tka_kvq_flash_decode_args* a) {
+  if (check_decode(a) != TKA_OK) return 0;
+  return partial_bytes((int64_t)a->cache.batch * a->cache.num_kv_heads * a->group, plan_decode(a));
+}
+
+int tka_kvq_flash_decode(const tka_kvq_flash_decode_args* a) {
+  const int rc = check_decode(a);
+  if (rc != TKA_OK) return rc;
+  if (!a->workspace || a->workspace_bytes < tka_kvq_flash_decode_workspace_bytes(a)) return TKA_EWORKSPACE;
+  KvAttendParams p;
+  memset(&p, 0, sizeof p);
+  p.q = a->q;
+  p.q_stride_b = a->q_stride_b;
+  p.batch = a->cache.batch;
+  p.num_kv_heads = a->cache.num_kv_heads;
+  p.group_log2 = log2_of(a->group);
+  p.own = rows_of(a->cache);
+  p.own_len = a->kv_len;
+  p.kv_idx = a->kv_idx;
+  p.kv_count = a->kv_count;
+  p.idx_len = a->idx_len;
+  p.out = a->out;
+  p.out_lse = a->out_lse;
+  p.out_stride_b = a->out_stride_b;
+  p.out_dtype = a->out_dtype;
+  p.scale_log2e = a->scale * 1.44269504088896340736f;
+  return run_attend(p, plan_decode(a), a->dtype, a->cache.format, a->workspace, (hipStream_t)a->stream);
+}
+
+size_t tka_prefix_decode_workspace_bytes(const tka_prefix_decode_args* a) {
+  if (check_prefix(a) != TKA_OK) return 0;
+  return partial_bytes((int64_t)a->suffix.batch * a->suffix.num_kv_heads * a->group, plan_prefix(a));
+}
+
+int tka_prefix_decode(const tka_prefix_decode_args* a) {
+  const int rc = check_prefix(a);
+  if (rc != TKA_OK) return rc;
+  if (!a->workspace || a->workspace_bytes < tka_prefix_decode_workspace_bytes(a)) return TKA_EWORKSPACE;
+  KvAttendParams p;
+  memset(&p, 0, sizeof p);
+  p.q = a->q;
+  p.q_stride_b = a->q_stride_b;
+  p.batch = a->suffix.batch;
+  p.num_kv_heads = a->suffix.num_kv_heads;
+  p.group_log2 = log2_of(a->group);
+  if (a->prefix.rows) p.shared = rows_of(a->prefix);
+  if (a->suffix.rows) p.own = rows_of(a->suffix);
+  p.own_len = a->suffix_len;
+  p.out = a->out;
+  p.out_lse = a->out_lse;
+  p.out_stride_b = a->out_stride_b;
+  p.out_dtype = a->out_dtype;
+  p.scale_log2e = a->scale * 1.44269504088896340736f;
+  return run_attend(p, plan_prefix(a), a->dtype, a->prefix.format, a->workspace, (hipStream_t)a->stream);
+}
+
+}  // extern "C"

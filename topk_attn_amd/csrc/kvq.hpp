@@ -1,0 +1,76 @@
+// Parameter blocks and launch functions of the 8-bit K/V cache and of the shared-prefix attention (internal).
+#pragma once
+#include "../../include/topk_attn_kvq.h"
+#include "common.hpp"
+
+namespace tka {
+
+// Strides of code rows are in BYTES, those of scales in elements; a stride of 0 shares the cache among the batch.
+struct KvRows {
+  const unsigned char* k;
+  const unsigned char* v;
+  const float* ks;
+  const float* vs;
+  int64_t stride_b, stride_n, stride_h;
+  int64_t scale_b, scale_n, scale_h;
+  int64_t rows;
+};
+
+// tka_kvq_write / tka_kvq_read: `in` side and `cache` side of the copy (the read goes the other way)
+struct KvqCopyParams {
+  KvRows cache;             // (its pointers are written by the write kernel)
+  unsigned char* k;         // 16-bit rows; strides in bytes
+  unsigned char* v;
+  int64_t stride_b, stride_n, stride_h;
+  const int32_t* start;
+  const int32_t* count;
+  int batch, num_kv_heads, num_tokens;
+  int tile_log2;            // a workgroup covers 2^tile_log2 tokens of each of 32 >> tile_log2 (entry, head) pairs (set by the launcher)
+};
+int launch_kvq_write(const KvqCopyParams& p, int dtype, int format, hipStream_t stream);
+int launch_kvq_read(const KvqCopyParams& p, int dtype, int format, hipStream_t stream);
+
+struct KvqScoresParams {
+  KvRows cache;
+  const void* q;
+  int64_t q_stride_b;
+  const int32_t* kv_len;
+  float* scores;
+  int batch, num_kv_heads, group;
+  float scale;
+};
+int launch_kvq_scores(const KvqScoresParams& p, int dtype, int format, hipStream_t stream);
+
+// Attention over up to two sources: `shared`, whose rows every query row of the batch attends to, and `own`, whose
+// entry b the queries of entry b attend to.  The grid is the shared items, then the own items.
+struct KvAttendParams {
+  const void* q;
+  int64_t q_stride_b;
+  int batch, num_kv_heads, group_log2;
+  KvRows shared;
+  int shared_splits;        // 0: no shared rows
+  int shared_tps;           // tokens per split, a multiple of kAttendTile
+  int row_blocks;           // query rows of a head (batch * group) in blocks of 16 * RT
+  KvRows own;
+  int own_splits;           // 0: no own rows
+  int own_tps;
+  const int32_t* own_len;   // [batch] or nullptr
+  const int32_t* kv_idx;    // [batch][num_kv_heads][idx_len] or nullptr
+  const int32_t* kv_count;  // [batch][num_kv_heads] or nullptr
+  int idx_len;
+  int num_splits;           // partials per query row: shared_splits + own_splits
+  float* part_m;            // [rows][num_splits], base-2 maxima
+  float* part_l;
+  float* part_acc;          // [rows][num_splits][128]
+  void* out;                // written here when num_splits == 1, else by the combine launch
+  float* out_lse;
+  int64_t out_stride_b;
+  int out_dtype;
+  float scale_log2e;
+};
+constexpr int kAttendTile = 32;   // tokens of a wave's tile
+int launch_kv_attend(const KvAttendParams& p, int dtype, int format, int row_tiles, hipStream_t stream);
+// Joins the partials of the query rows and writes p.out / p.out_lse (num_splits > 1).
+int launch_kv_combine(const KvAttendParams& p, hipStream_t stream);
+
+}  // namespace tka

@@ -383,6 +383,336 @@ def sparse_decode_step(q, keys, values, k, sink, local, scale, group, out_dtype=
     return plan.out, plan.topk_idx, plan.topk_val, plan.union_idx, plan.union_count
 
 
+# ---- 8-bit K/V caches and shared prefixes (include/topk_attn_kvq.h) --------------------------------
+
+_KV_FORMAT = {torch.float8_e4m3fn: L.TKA_KV_E4M3, torch.int8: L.TKA_KV_INT8}
+
+
+def _one_device(*tensors):
+    """Index of the GPU that all the tensors (None aside) live on."""
+    _need_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError("tensors must live on one GPU, got %s" % sorted(map(str, devices)))
+    return devices.pop().index
+
+
+def _call(fn, args, device, where):
+    """One C call on the current stream of `device` (which need not be the current device)."""
+    if torch.cuda.current_device() == device:
+        args.stream = torch.cuda.current_stream().cuda_stream
+        rc = fn(C.byref(args))
+    else:
+        with torch.cuda.device(device):
+            args.stream = torch.cuda.current_stream().cuda_stream
+            rc = fn(C.byref(args))
+    if rc != L.TKA_OK:
+        L.check(rc, where)
+
+
+def _need_workspace(need, fn, args, where):
+    """The C side's reason for a workspace size of zero (its checks come before any launch)."""
+    if need == 0:
+        L.check(fn(C.byref(args)) or L.TKA_EINVAL, where)
+
+
+def _strides(t, dims):
+    """Strides of a tensor's dims in elements; a dim of size 1 has none that matters."""
+    return [0 if t.shape[d] == 1 else t.stride(d) for d in dims]
+
+
+def _alike(a, b):
+    """Same shape, and the same strides where they matter."""
+    return a.shape == b.shape and _strides(a, range(a.dim())) == _strides(b, range(b.dim()))
+
+
+def _int32(t, shape, name):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError("%s must be int32 %s, contiguous" % (name, list(shape)))
+    return t
+
+
+def _rows4(t, name):
+    """[N,H,128] (shared by a batch) or [B,N,H,128] with contiguous rows -> the 4-dim view."""
+    if t.dim() not in (3, 4) or t.shape[-1] != 128 or t.stride(-1) != 1:
+        raise ValueError("%s must be [N,H,128] or [B,N,H,128] with a contiguous last dim" % name)
+    return t if t.dim() == 4 else t.unsqueeze(0)
+
+
+def _fill_cache(c, fmt, k, v, batch, shared):
+    """tka_kv_cache of 4-dim tensors; `shared`: entry 0 serves every entry of the batch."""
+    c.k, c.v, c.format = k.data_ptr(), (v.data_ptr() if v is not None else None), fmt
+    c.batch, c.rows, c.num_kv_heads, c.head_dim = batch, k.shape[1], k.shape[2], 128
+    c.stride_b, c.stride_n, c.stride_h = _strides(k, (0, 1, 2))
+    if shared:
+        c.stride_b = 0
+
+
+class QuantCache:
+    """K/V cache of 8-bit rows: codes [B,N,H,128] (or [N,H,128], one cache that a batch shares) in torch.float8_e4m3fn or
+    torch.int8 - the dtype names the format - and one fp32 scale per row, [B,N,H] (or [N,H]).  Any strides with 16-byte
+    aligned rows; keys and values share theirs.  v_codes / v_scale may be None where only scores are taken."""
+
+    def __init__(self, k_codes, v_codes, k_scale, v_scale):
+        self.device = _one_device(k_codes, v_codes, k_scale, v_scale)
+        if k_codes.dtype not in _KV_FORMAT:
+            raise TypeError("codes must be float8_e4m3fn or int8, got %s" % k_codes.dtype)
+        self.shared = k_codes.dim() == 3
+        if (v_codes is None) != (v_scale is None):
+            raise ValueError("v_codes and v_scale go together")
+        for codes, scale, name in ((k_codes, k_scale, "k"), (v_codes, v_scale, "v")):
+            if codes is None:
+                continue
+            _rows4(codes, name + "_codes")
+            if codes.dtype != k_codes.dtype or not _alike(codes, k_codes):
+                raise ValueError("keys and values must share dtype, shape and strides")
+            if scale.dtype != torch.float32 or scale.shape != codes.shape[:-1]:
+                raise ValueError("%s_scale must be float32 %s" % (name, list(codes.shape[:-1])))
+            if not _alike(scale, k_scale):
+                raise ValueError("the scales of keys and values must share strides")
+        self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
+        self.format = _KV_FORMAT[k_codes.dtype]
+        self.batch = 1 if self.shared else k_codes.shape[0]
+        self.rows, self.heads = k_codes.shape[-3], k_codes.shape[-2]
+
+    @classmethod
+    def empty(cls, batch, rows, heads, dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache of zeros for `batch` entries of `rows` tokens, head by head (a head's rows and scales are contiguous:
+        the layout that the kernels stream best).  batch None: one cache [N,H,128] that a batch shares."""
+        n = 1 if batch is None else batch
+        codes = [torch.zeros((n, heads, rows, 128), dtype=torch.uint8, device=device).view(dtype).transpose(1, 2) for _ in range(2)]
+        scale = [torch.zeros((n, heads, rows), dtype=torch.float32, device=device).transpose(1, 2) for _ in range(2)]
+        if batch is None:
+            codes, scale = [c[0] for c in codes], [s[0] for s in scale]
+        return cls(codes[0], codes[1], scale[0], scale[1])
+
+    def _fill(self, c, batch):
+        """The C description for a call of `batch` entries."""
+        if not self.shared and self.batch != batch:
+            raise ValueError("batch mismatch: cache %d, call %d" % (self.batch, batch))
+        k, ks = (self.k_codes, self.k_scale) if not self.shared else (self.k_codes.unsqueeze(0), self.k_scale.unsqueeze(0))
+        _fill_cache(c, self.format, k, self.v_codes, batch, self.shared)
+        c.k_scale, c.v_scale = ks.data_ptr(), (self.v_scale.data_ptr() if self.v_scale is not None else None)
+        c.scale_stride_b, c.scale_stride_n, c.scale_stride_h = _strides(ks, (0, 1, 2))
+        if self.shared:
+            c.scale_stride_b = 0
+
+    def _need_values(self):
+        if self.v_codes is None:
+            raise ValueError("this call needs the values of the cache")
+
+
+class _KvqCopyPlan:
+    """What the write and the read plan share: rows k, v [B,T,H,128] on the 16-bit side."""
+
+    def __init__(self, args, fn, where, cache, k, v, start, count):
+        cache._need_values()
+        self._device = _one_device(cache.k_codes, k, v, start, count)
+        for t in (k, v):
+            if t.dim() != 4 or t.shape[-1] != 128 or t.stride(-1) != 1:
+                raise ValueError("k and v must be [B,T,H,128] with a contiguous last dim")
+        B, T, H, _ = k.shape
+        if v.dtype != k.dtype or not _alike(k, v):
+            raise ValueError("k and v must share dtype, shape and strides")
+        if H != cache.heads or B != cache.batch:
+            raise ValueError("k and v do not match the cache's batch entries or heads")
+        self.cache, self.k, self.v = cache, k, v
+        self.start, self.count = _int32(start, (B,), "start"), _int32(count, (B,), "count")
+        a = self.args = args
+        cache._fill(a.cache, B)
+        a.k, a.v, a.dtype, a.num_tokens = k.data_ptr(), v.data_ptr(), _dtype_code(k), T
+        a.stride_b, a.stride_n, a.stride_h = _strides(k, (0, 1, 2))
+        a.start = start.data_ptr() if start is not None else None
+        a.count = count.data_ptr() if count is not None else None
+        self._fn, self._where = fn, where
+
+    def run(self):
+        _call(self._fn, self.args, self._device, self._where)
+        return self
+
+
+class KvqWritePlan(_KvqCopyPlan):
+    """Quantises rows k, v [B,T,H,128] into a QuantCache: row t of entry b goes to row start[b] + t (start None: 0) for
+    t < count[b] (None: T); start and count are int32 [B] on the GPU.  run() is one C call; what k, v, start and count
+    hold when it runs counts."""
+
+    def __init__(self, cache, k, v, start=None, count=None):
+        super().__init__(L.KvqWriteArgs(), L.lib().tka_kvq_write, "tka_kvq_write", cache, k, v, start, count)
+
+
+class KvqReadPlan(_KvqCopyPlan):
+    """The other way: rows start[b] + t of a QuantCache as 16-bit numbers in k, v [B,T,H,128]; rows behind count[b], and
+    rows that the cache does not have, keep what they hold."""
+
+    def __init__(self, cache, k, v, start=None, count=None):
+        super().__init__(L.KvqReadArgs(), L.lib().tka_kvq_read, "tka_kvq_read", cache, k, v, start, count)
+
+
+def kvq_write(cache, k, v, start=None, count=None):
+    """Quantise k, v [B,T,H,128] into a QuantCache (see KvqWritePlan)."""
+    KvqWritePlan(cache, k, v, start, count).run()
+    return cache
+
+
+def kvq_read(cache, num_tokens, start=None, count=None, dtype=torch.bfloat16):
+    """Rows of a QuantCache as 16-bit numbers: (k, v) [B,num_tokens,H,128], zeros where there is no row."""
+    cache._need_values()
+    shape = (cache.batch, num_tokens, cache.heads, 128)
+    k, v = (torch.zeros(shape, dtype=dtype, device=cache.k_codes.device) for _ in range(2))
+    KvqReadPlan(cache, k, v, start, count).run()
+    return k, v
+
+
+class KvqScoresPlan:
+    """Stage-1 scores over the keys of a QuantCache: scores fp32 [B,Hkv,N], -inf behind kv_len[b] (int32 [B] on the GPU;
+    None: all rows).  What topk() selects from; run() is one C call."""
+
+    def __init__(self, q, cache, scale=1.0, group=1, kv_len=None):
+        self._device = _one_device(q, cache.k_codes, kv_len)
+        q = _q3(q)
+        B = q.shape[0]
+        if q.shape[1] != cache.heads * group:
+            raise ValueError("q heads != kv heads * group")
+        self.q, self.cache, self.kv_len = q, cache, _int32(kv_len, (B,), "kv_len")
+        a = self.args = L.KvqScoresArgs()
+        cache._fill(a.cache, B)
+        a.q, a.dtype, a.group, a.q_stride_b, a.scale = q.data_ptr(), _dtype_code(q), group, _strides(q, (0,))[0], scale
+        a.kv_len = kv_len.data_ptr() if kv_len is not None else None
+        self.scores = torch.empty((B, cache.heads, cache.rows), dtype=torch.float32, device=q.device)
+        a.out_scores = self.scores.data_ptr()
+        self._fn = L.lib().tka_kvq_scores
+
+    def run(self):
+        _call(self._fn, self.args, self._device, "tka_kvq_scores")
+        return self
+
+
+def kvq_scores(q, cache, scale=1.0, group=1, kv_len=None):
+    """Scores fp32 [B,Hkv,N] over a QuantCache's keys (see KvqScoresPlan)."""
+    return KvqScoresPlan(q, cache, scale, group, kv_len).run().scores
+
+
+class _DecodeOutputs:
+    """Outputs and workspace of a decode plan."""
+
+    def _finish(self, a, q, out_dtype, return_lse, need, fn, where):
+        B, Hq, _ = q.shape
+        if out_dtype not in _DT:
+            raise TypeError("expected float16 or bfloat16, got %s" % out_dtype)
+        self.out = torch.empty((B, Hq, 128), dtype=out_dtype, device=q.device)
+        self.lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+        a.out, a.out_dtype, a.out_stride_b = self.out.data_ptr(), _DT[out_dtype], Hq * 128
+        a.out_lse = self.lse.data_ptr() if return_lse else None
+        size = need(C.byref(a))
+        _need_workspace(size, fn, a, where)
+        self.ws = _own_workspace(size, q.device)
+        a.workspace, a.workspace_bytes = self.ws.data_ptr(), self.ws.numel()
+        self._fn, self._where = fn, where
+
+    def run(self):
+        _call(self._fn, self.args, self._device, self._where)
+        return self
+
+
+class KvqFlashDecodePlan(_DecodeOutputs):
+    """Argument block, output and workspace of one decode step of attention over a QuantCache: over its first kv_len[b]
+    rows (int32 [B]; None: all), or over the rows listed in kv_idx int32 [B,Hkv,L] (the first kv_count[b,h] entries of
+    each list; ids outside the cache or behind kv_len are skipped).  A query without a row gets zeros, its lse is -inf.
+    run() is one C call; a plan runs on one stream at a time."""
+
+    def __init__(self, q, cache, scale, group=1, num_splits=0, kv_len=None, kv_idx=None, kv_count=None, out_dtype=None,
+                 return_lse=False):
+        cache._need_values()
+        self._device = _one_device(q, cache.k_codes, kv_len, kv_idx, kv_count)
+        q = _q3(q)
+        B, H = q.shape[0], cache.heads
+        if q.shape[1] != H * group:
+            raise ValueError("q heads != kv heads * group")
+        if kv_idx is not None and (kv_idx.dim() != 3 or kv_idx.shape[-1] < 1):
+            raise ValueError("kv_idx must be int32 [B,Hkv,L]")
+        self.q, self.cache = q, cache
+        self.kv_len = _int32(kv_len, (B,), "kv_len")
+        self.kv_idx = _int32(kv_idx, (B, H, kv_idx.shape[-1] if kv_idx is not None else 0), "kv_idx")
+        self.kv_count = _int32(kv_count, (B, H), "kv_count")
+        a = self.args = L.KvqFlashDecodeArgs()
+        cache._fill(a.cache, B)
+        a.q, a.dtype, a.group, a.q_stride_b = q.data_ptr(), _dtype_code(q), group, _strides(q, (0,))[0]
+        a.num_splits, a.scale = num_splits, scale
+        a.kv_len = kv_len.data_ptr() if kv_len is not None else None
+        if kv_idx is not None:
+            a.kv_idx, a.idx_len = kv_idx.data_ptr(), kv_idx.shape[-1]
+        a.kv_count = kv_count.data_ptr() if kv_count is not None else None
+        self._finish(a, q, out_dtype or q.dtype, return_lse, L.lib().tka_kvq_flash_decode_workspace_bytes,
+                     L.lib().tka_kvq_flash_decode, "tka_kvq_flash_decode")
+
+
+def kvq_flash_decode(q, cache, scale, group=1, num_splits=0, kv_len=None, kv_idx=None, kv_count=None, out_dtype=None,
+                     return_lse=False):
+    """Decode attention over a QuantCache (see KvqFlashDecodePlan).  Returns out [B,Hq,128] (and lse fp32 [B,Hq])."""
+    plan = KvqFlashDecodePlan(q, cache, scale, group, num_splits, kv_len, kv_idx, kv_count, out_dtype, return_lse).run()
+    return (plan.out, plan.lse) if return_lse else plan.out
+
+
+class PrefixDecodePlan(_DecodeOutputs):
+    """One decode step of a batch whose sequences share a prefix and go on with a suffix each: the prefix is read once for
+    the batch.  prefix and suffix are QuantCaches of one dtype, or pairs (keys, values) of 16-bit tensors of q's dtype:
+    the prefix [P,H,128] (or a batch of one), the suffix [B,S,H,128].  Either may be None.  suffix_len: int32 [B], the rows
+    of each suffix (None: S).  run() is one C call; a plan runs on one stream at a time."""
+
+    def __init__(self, q, prefix, suffix, scale, group=1, suffix_len=None, num_splits=0, out_dtype=None, return_lse=False):
+        q = _q3(q)
+        B = q.shape[0]
+        a = self.args = L.PrefixDecodeArgs()
+        if prefix is None and suffix is None:
+            raise ValueError("neither a prefix nor a suffix")
+        tensors, formats = [q, suffix_len], set()
+        for source, c, name, batch in ((prefix, a.prefix, "prefix", 1), (suffix, a.suffix, "suffix", B)):
+            if source is None:
+                continue
+            if isinstance(source, QuantCache):
+                source._need_values()
+                if name == "suffix" and source.shared:
+                    raise ValueError("the suffix must be [B,S,H,128]")
+                source._fill(c, batch)
+                tensors += [source.k_codes, source.v_codes]
+            else:
+                k, v = source
+                if k.dtype != q.dtype or v.dtype != q.dtype:
+                    raise TypeError("16-bit caches must have q's dtype")
+                if not _alike(k, v):
+                    raise ValueError("keys and values must share shape and strides")
+                if name == "suffix" and k.dim() != 4:
+                    raise ValueError("the suffix must be [B,S,H,128]")
+                k4 = _rows4(k, name)
+                if k4.shape[0] != batch:
+                    raise ValueError("%s: batch mismatch" % name)
+                _fill_cache(c, L.TKA_KV_16BIT, k4, v, batch, False)
+                tensors += [k, v]
+            if q.shape[1] != c.num_kv_heads * group:
+                raise ValueError("q heads != kv heads * group")
+            formats.add(c.format)
+        if len(formats) != 1:
+            raise ValueError("prefix and suffix must have one format")
+        for source, c, batch in ((prefix, a.prefix, 1), (suffix, a.suffix, B)):
+            if source is None:
+                c.format, c.batch, c.rows, c.num_kv_heads, c.head_dim = formats.copy().pop(), batch, 0, q.shape[1] // group, 128
+        self._device = _one_device(*tensors)
+        self.q, self.prefix, self.suffix, self.suffix_len = q, prefix, suffix, _int32(suffix_len, (B,), "suffix_len")
+        a.q, a.dtype, a.group, a.q_stride_b = q.data_ptr(), _dtype_code(q), group, _strides(q, (0,))[0]
+        a.num_splits, a.scale = num_splits, scale
+        a.suffix_len = suffix_len.data_ptr() if suffix_len is not None else None
+        self._finish(a, q, out_dtype or q.dtype, return_lse, L.lib().tka_prefix_decode_workspace_bytes,
+                     L.lib().tka_prefix_decode, "tka_prefix_decode")
+
+
+def prefix_decode(q, prefix, suffix, scale, group=1, suffix_len=None, num_splits=0, out_dtype=None, return_lse=False):
+    """Decode attention of a batch behind a shared prefix (see PrefixDecodePlan).  Returns out [B,Hq,128] (and lse)."""
+    plan = PrefixDecodePlan(q, prefix, suffix, scale, group, suffix_len, num_splits, out_dtype, return_lse).run()
+    return (plan.out, plan.lse) if return_lse else plan.out
+
+
 def set_test_hooks(force_segment_redo=0, tau_spin_limit=0, tau_withhold_mod=0, tau_withhold_rem=0, tau_withhold_mode=0,
                    union_handoff_order=0, fused_tail=0):
     """Testing hooks (see tka_test_hooks in include/topk_attn.h); no arguments = defaults."""
