@@ -166,6 +166,7 @@ template <int DT, int FMT, int RT, bool INDEXED>
 __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem& it, AttendLds& sh) {
   constexpr bool kQF16 = DT == TKA_F16;
   constexpr bool kPF16 = kQuantised<FMT> || DT == TKA_F16;   // type of the second product
+  constexpr bool kSplit = !kPF16 || DT == TKA_F16;           // weights in two parts
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int n = lane & 15, j = lane >> 4;
   const int group = 1 << p.group_log2;
@@ -315,10 +316,15 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float a = ps[2 * w], b = ps[2 * w + 1];
-          if constexpr (kQuantised<FMT>) {
-            pf[r][w] = pack_f16(a * weight[2 * w], b * weight[2 * w + 1]);
-          } else if constexpr (kPF16) {
-            pf[r][w] = pack_f16(a, b);
+          if constexpr (kPF16) {
+            const float x = kQuantised<FMT> ? a * weight[2 * w] : a, y = kQuantised<FMT> ? b * weight[2 * w + 1] : b;
+            pf[r][w] = pack_f16(x, y);
+            if constexpr (kSplit) {
+              uint32_t hi = pf[r][w];
+              asm("" : "+v"(hi));   // (the compiler otherwise folds the conversions into mixed-precision multiply-adds and takes the first pair's rounded weights for all four)
+              const f16x2 h = __builtin_bit_cast(f16x2, hi);
+              pf_lo[r][w] = pack_f16(x - (float)h[0], y - (float)h[1]);
+            }
           } else {
             pf[r][w] = pack_bf16(a, b);
             pf_lo[r][w] = pack_bf16(a - __builtin_bit_cast(float, pf[r][w] << 16), b - __builtin_bit_cast(float, pf[r][w] & 0xffff0000u));
@@ -335,9 +341,9 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
       for (int r = 0; r < RT; ++r) {
         acc[r][2 * D] = mfma<kPF16>(even, pf[r], acc[r][2 * D]);
         acc[r][2 * D + 1] = mfma<kPF16>(odd, pf[r], acc[r][2 * D + 1]);
-        if constexpr (!kPF16) {
-          acc[r][2 * D] = mfma<false>(even, pf_lo[r], acc[r][2 * D]);
-          acc[r][2 * D + 1] = mfma<false>(odd, pf_lo[r], acc[r][2 * D + 1]);
+        if constexpr (kSplit) {
+          acc[r][2 * D] = mfma<kPF16>(even, pf_lo[r], acc[r][2 * D]);
+          acc[r][2 * D + 1] = mfma<kPF16>(odd, pf_lo[r], acc[r][2 * D + 1]);
         }
       }
     };
