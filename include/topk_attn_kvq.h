@@ -39,7 +39,8 @@ typedef enum tka_kv_format {
  * k + (b*stride_b + t*stride_n + h*stride_h) elements (one byte each in the 8-bit formats, two in TKA_KV_16BIT), its scale
  * is k_scale[b*scale_stride_b + t*scale_stride_n + h*scale_stride_h]; values likewise with the same strides.  Rows are
  * 16-byte aligned.  Tokens that lie next to each other in a head's scales (scale_stride_n = 1) are what the kernels
- * read best; codes may lie token by token or head by head. */
+ * read best; codes may lie token by token or head by head.  The attention entry points take rows of a head, and
+ * scales, up to 64 MiB apart (TKA_EUNSUPPORTED beyond). */
 typedef struct tka_kv_cache {
   void* k;
   void* v;                /* may be NULL where only keys are read (tka_kvq_scores)              */

@@ -12,16 +12,20 @@
 //
 // 8-bit rows: a code is exact as a 16-bit number, so K codes go to the type of q and V codes to fp16; the scale of a key
 // row multiplies its logits, that of a value row its weight, both in fp32.  Weights enter the second product as fp16:
-// p * (scale / cap) * 2^14, with cap a power of two no scale seen so far exceeds (accumulators move with it), so that a
-// weight is rounded by 2^-11 of itself down to 2^-28 of the largest, and by 2^-39 of that below.  16-bit rows: fp16
-// weights are held the same way without a cap; bf16 weights have fp32's range but 8 bits only, the remainder goes through
-// the matrix cores as a second operand, and they are held times 2^-32, so that no sum of the largest numbers overflows.
-// (The factor sits in the exponent, and the sum of the weights has it too.)
+// 2^(x - m) * (scale / cap) * 2^9, with cap a power of two no scale seen so far exceeds (accumulators move with it) and m a
+// reference that no logit x exceeds by more than 6: at most 2^15, rounded by 2^-11 of themselves down to 2^-14 and by 2^-25
+// below.  Where q is fp16 the remainder goes through the matrix cores as a second operand, so that the weights are as
+// exact as the output.  16-bit rows: fp16 weights are held the same way without a cap; bf16 weights have fp32's range but
+// 8 bits only, their remainder always is a second operand, and they are held times 2^-32, so that no sum of the largest
+// numbers overflows.  (The factor sits in the exponent, and the sum of the weights has it too.)
+//
+// The reference m of a row only moves when weights have grown by 2^6: after the first tiles that is rare, and a tile then
+// needs neither the row's maximum, an exchange between lanes, nor a pass over the accumulators.
 //
 // Results of waves and splits are joined normalised, out = sum (l_s 2^(m_s - M) / L) o_s: they stay in the range of V.
 //
 // A workgroup is one (source, batch entry or block of query rows, head, split); its waves take 32-token tiles in turn and
-// are joined in LDS.  The shared source multiplies a block of 16 * RT query rows (entries x group) with each K / V tile.
+// are joined in LDS, the splits by a second launch.  The shared source multiplies a block of 16 * RT query rows (entries x group) with each K / V tile.
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -32,10 +36,13 @@ namespace tka {
 namespace {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kTile = kAttendTile;
+constexpr float kNoReference = -3.402823466e38f;   // of a row that has seen no key: what lies above it moves it
+constexpr int kStagedIds = 2048;
 constexpr int kLdsRow = kHeadDim + 4;   // (rows 4 floats apart in the banks)
 
 __device__ __forceinline__ f32x4 mfma_f16(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -139,46 +146,71 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
   return x + __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, x)));
 }
 
+constexpr int kJoined = 4;   // waves that are joined in one go
 struct AttendLds {
-  float acc[kWaves][16][kLdsRow];
-  float m[kWaves][16];
-  float l[kWaves][16];
+  float acc[kJoined][16][kLdsRow];
+  union {
+    struct {
+      float m[kJoined][16];
+      float l[kJoined][16];
+    };
+    float state[kJoined][kWave][3];   // of more than four waves: reference, sum, cap
+  };
 };
 
 template <bool F16>
-constexpr float kWeightLog2 = F16 ? 14.0f : -32.0f;   // weights are held times 2^this
+constexpr float kWeightLog2 = F16 ? 9.0f : -32.0f;   // weights are held times 2^this
+template <bool F16>
+constexpr float kMostWeight = F16 ? 32768.0f : 0x1p-26f;   // 2^6 times that: the reference moves when eight weights add up to more
 
-// What a workgroup attends to: positions [begin, end) of a source (of its token list where there is one) for the query
-// rows [row0, row0 + 16 RT) below row_end; query row r is head h * group + r % group of batch entry b0 + r / group.
-struct AttendItem {
-  const unsigned char* k;   // of the entry and head
+// Positions [begin, end) of the rows of one entry and head (of a token list where there is one).
+struct AttendSource {
+  const unsigned char* k;
   const unsigned char* v;
   const float* ks;
   const float* vs;
   int64_t stride_n, scale_n;
   const int32_t* idx;
-  int64_t len;              // rows of the cache that listed ids may name
-  int64_t begin, end;
+  int len;                  // rows of the cache that listed ids may name
+  int begin, end;           // (uniform over the wave, like everything here)
+};
+
+// What a workgroup attends to, one source after the other, for the query rows [row0, row0 + 16 RT) below row_end; query row
+// r is head h * group + r % group of batch entry b0 + r / group.
+struct AttendItem {
+  AttendSource first, second;
+  bool two;
   int b0, h, row0, row_end, slot;
 };
 
-template <int DT, int FMT, int RT, bool INDEXED>
-__device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem& it, AttendLds& sh) {
+// Dims d0 .. d0+7 of a finished row (query head hq of entry b) and, with the first of them, its lse.
+__device__ __forceinline__ void store_row(const KvAttendParams& p, int b, int hq, int d0, const f32x4& lo, const f32x4& hi, float M, float L, float l_log2) {
+  u32x4 o;
+  if (p.out_dtype == TKA_F16) o = (u32x4){pack_f16(lo[0], lo[1]), pack_f16(lo[2], lo[3]), pack_f16(hi[0], hi[1]), pack_f16(hi[2], hi[3])};
+  else o = (u32x4){pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3])};
+  *(u32x4*)((uint16_t*)p.out + b * p.out_stride_b + (int64_t)hq * kHeadDim + d0) = o;
+  if (p.out_lse && d0 == 0)
+    p.out_lse[(((int64_t)b * p.num_kv_heads) << p.group_log2) + hq] = L > 0.0f || L != L ? (M + (__builtin_log2f(L) - l_log2)) * 0.69314718055994531f : -INFINITY;
+}
+
+template <int DT, int FMT, int RT, bool INDEXED, int WAVES>
+__device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem& item, AttendLds& sh, int32_t* sh_ids) {
   constexpr bool kQF16 = DT == TKA_F16;
   constexpr bool kPF16 = kQuantised<FMT> || DT == TKA_F16;   // type of the second product
   constexpr bool kSplit = !kPF16 || DT == TKA_F16;           // weights in two parts
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, j = lane >> 4;
   const int group = 1 << p.group_log2;
 
   u32x4 qf[RT][4];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int row = it.row0 + 16 * r + n;
-    const bool there = row < it.row_end;
+    const int row = item.row0 + 16 * r + n;
+    const bool there = row < item.row_end;
     const int rr = there ? row : 0;
-    const uint16_t* q = (const uint16_t*)p.q + (int64_t)(it.b0 + (rr >> p.group_log2)) * p.q_stride_b +
-                        (int64_t)(it.h * group + (rr & (group - 1))) * kHeadDim;
+    const uint16_t* q = (const uint16_t*)p.q + (int64_t)(item.b0 + (rr >> p.group_log2)) * p.q_stride_b +
+                        (int64_t)(item.h * group + (rr & (group - 1))) * kHeadDim;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
       qf[r][kb] = *(const u32x4*)(q + k_dim<FMT>(kb, j));
@@ -186,97 +218,127 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
     }
   }
 
-  float m_run[RT], l_run[RT];   // of query row n of each tile; l_run: this quarter's share
+  float m_ref[RT], l_run[RT];   // of query row n of each tile; l_run: this quarter's share
   f32x4 acc[RT][8];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    m_run[r] = -INFINITY;
+    m_ref[r] = kNoReference;
     l_run[r] = 0.0f;
 #pragma unroll
     for (int c = 0; c < 8; ++c) acc[r][c] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
   float cap = __builtin_bit_cast(float, 17u << 23);   // 2^-110: the least cap (its reciprocal stays in range)
 
-  const unsigned char* kb_base = it.k + 16 * j;
-  const unsigned char* vb_base = it.v + (kQuantised<FMT> ? 8 : 16) * n;
-
-  for (int64_t tile = it.begin + wave * kTile; tile < it.end; tile += kWaves * kTile) {
-    const bool full = tile + kTile <= it.end;
-    int64_t tk[2], tv[8];
-    bool ok[8];
-    bool skipped = false;
+  // One source: its tiles go round the waves, `turn` is this wave's first.
+  const auto attend_source = [&](const AttendSource& it, int turn) {
+  KTile<FMT> kt[2];
+  VRow<FMT> vr[8];
+  float ks[8], vs[8];
+  // Rows of a tile of 32 positions from `start`: key rows 16x + n, value and scale rows the slot tokens.  Dense: a scalar
+  // base and 32-bit lane offsets (32 strides fit, the host checks), rows that a source of less than 32 does not have
+  // replaced by its last.  Listed: the ids of the positions, -1 replaced by row 0.
+  uint32_t k_off[2], v_off[8];
+  const bool vector_scales = it.scale_n == 1 && it.end >= kTile;
+  if constexpr (!INDEXED) {
+    const uint32_t stride = (uint32_t)it.stride_n;
+    const int last = min(it.end, kTile) - 1;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int64_t pos = tile + 16 * x + n;
-      const int64_t pc = pos < it.end ? pos : it.end - 1;
-      int64_t t = INDEXED ? (int64_t)it.idx[pc] : pc;
-      if (INDEXED && (t < 0 || t >= it.len)) t = 0;
-      tk[x] = t;
-    }
+    for (int x = 0; x < 2; ++x) k_off[x] = (uint32_t)min(16 * x + n, last) * stride + 16u * j;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const int64_t pos = tile + slot_token(j, s);
-      ok[s] = pos < it.end;
-      const int64_t pc = ok[s] ? pos : it.end - 1;
-      int64_t t = INDEXED ? (int64_t)it.idx[pc] : pc;
-      if (INDEXED && (t < 0 || t >= it.len)) {
-        ok[s] = false;
-        t = 0;
-        skipped = true;
+    for (int s = 0; s < 8; ++s) v_off[s] = (uint32_t)min(slot_token(j, s), last) * stride + (kQuantised<FMT> ? 8u : 16u) * n;
+  }
+  const auto load_scales = [&](const float* of_source, int start, float (&f)[8]) {
+    if constexpr (INDEXED) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 * x + i] = of_source[(int64_t)max(id[i], 0) * it.scale_n];
       }
-      tv[s] = t;
-    }
-    KTile<FMT> kt[2];
-    VRow<FMT> vr[8];
+    } else {
+      const float* base = of_source + (int64_t)start * it.scale_n;
+      if (vector_scales) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 2; ++x) {
+          const f32x4u v = *(const f32x4u*)(base + 16 * x + 4u * j);
 #pragma unroll
-      for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(kb_base + tk[x] * it.stride_n + 64 * y);
-#pragma unroll
-    for (int s = 0; s < 8; ++s) vr[s] = *(const VRow<FMT>*)(vb_base + tv[s] * it.stride_n);
-    float ks[8], vs[8];
-    if constexpr (kQuantised<FMT>) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        ks[s] = it.ks[tv[s] * it.scale_n];
-        vs[s] = it.vs[tv[s] * it.scale_n];
-      }
-    }
-    // rows of masked slots (behind the end, ids outside the cache) must not reach the products: 0 * inf, 0 * NaN
-    if (!full || (INDEXED && __ballot(skipped) != 0ull)) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-        if (!ok[s]) {
-          vr[s] = VRow<FMT>{};
-          if constexpr (kQuantised<FMT>) vs[s] = 0.0f;
+          for (int i = 0; i < 4; ++i) f[4 * x + i] = v[i];
         }
-    }
-    float weight[8];   // scale of a slot's value row over the cap
-    if constexpr (kQuantised<FMT>) {
-      float top = vs[0];
+      } else {
+        int last = min(it.end, kTile) - 1;
+        asm("" : "+s"(last));   // (the eight offsets are made here, not kept in registers over the loop)
 #pragma unroll
-      for (int s = 1; s < 8; ++s) top = fmaxf(top, vs[s]);
-      if (__ballot(top > cap) != 0ull) {
-        top = max_over_quarters(top);
-        const uint32_t e = (__builtin_bit_cast(uint32_t, top) + 0x7fffffu) & 0x7f800000u;   // the power of two at or above it
-        const float raised = __builtin_bit_cast(float, e < 0x7f000000u ? e : 0x7f000000u);
-        const float drop = cap / raised;
-        cap = raised;
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) acc[r][c] *= drop;
-      }
-      const float unit = 1.0f / cap;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        weight[s] = vs[s] * unit;
-        ks[s] *= p.scale_log2e;
+        for (int s = 0; s < 8; ++s) f[s] = *(const float*)((const unsigned char*)base + (uint32_t)min(slot_token(j, s), last) * (uint32_t)(4 * it.scale_n));
       }
     }
+  };
+  const auto load_keys = [&](int start) {
+    if constexpr (INDEXED) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const unsigned char* row = it.k + (int64_t)max(sh_ids[start + 16 * x + n], 0) * it.stride_n + 16 * j;
+#pragma unroll
+        for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(row + 64 * y);
+      }
+    } else {
+      const unsigned char* base = it.k + (int64_t)start * it.stride_n;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(base + k_off[x] + 64 * y);
+    }
+    if constexpr (kQuantised<FMT>) load_scales(it.ks, start, ks);
+  };
+  const auto load_values = [&](int start) {
+    if constexpr (INDEXED) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[4 * x + i] = *(const VRow<FMT>*)(it.v + (int64_t)max(id[i], 0) * it.stride_n + (kQuantised<FMT> ? 8 : 16) * n);
+      }
+    } else {
+      const unsigned char* base = it.v + (int64_t)start * it.stride_n;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) vr[s] = *(const VRow<FMT>*)(base + v_off[s]);
+    }
+    if constexpr (kQuantised<FMT>) load_scales(it.vs, start, vs);
+  };
 
-    u32x4 pf[RT], pf_lo[RT];
-    {
+  // Positions [begin, end): the waves take tiles in turn.  The keys of the next tile are asked for as soon as those of this
+  // one are in the matrix cores, its values behind this tile's.  A dense tile that the end cuts starts earlier, at the last
+  // 32 rows that there are, and its first positions are masked (listed positions are filled up with -1).
+  const auto run = [&](int begin, int end) {
+    int rest = end - begin - turn * kTile;   // positions from this tile's first on
+    if (rest <= 0) return;
+    int tile = begin + turn * kTile;
+    int start = INDEXED || rest >= kTile ? tile : max(end - kTile, 0);
+    load_keys(start);
+    load_values(start);
+    while (true) {
+      asm("" : "+s"(start));   // (addresses are made from it in scalar registers, not carried along in vector registers)
+      const bool more = rest > WAVES * kTile;
+      const int next_tile = tile + WAVES * kTile;
+      const int next = INDEXED || rest >= (WAVES + 1) * kTile ? next_tile : max(end - kTile, 0);
+      uint32_t masked = 0;   // bit s: slot s has no row
+      bool any_masked;
+      if constexpr (INDEXED) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) masked |= id[i] < 0 ? 1u << (4 * x + i) : 0u;
+        }
+        any_masked = __ballot(masked != 0) != 0ull;
+      } else {
+        any_masked = rest < kTile;
+        if (any_masked) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s) masked |= start + slot_token(j, s) < tile || start + slot_token(j, s) >= end ? 1u << s : 0u;
+        }
+      }
+
+      // ---- logits, before their scales
       f32x4 sc[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; ++r) sc[r][0] = sc[r][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -288,34 +350,81 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
 #pragma unroll
           for (int r = 0; r < RT; ++r) sc[r][x] = mfma<kQF16>(a, qf[r][kb], sc[r][x]);
         }
+      float kf[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) kf[s] = kQuantised<FMT> ? ks[s] * p.scale_log2e : p.scale_log2e;
+      if (more) load_keys(next);
+
+      // masked slots: no weight, and nothing of their rows in the products (0 * inf, 0 * NaN)
+      if (any_masked) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (masked >> s & 1u) {
+            vr[s] = VRow<FMT>{};
+            vs[s] = 0.0f;
+            kf[s] = 1.0f;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) sc[r][s >> 2][s & 3] = -INFINITY;
+          }
+      }
+      float weight[8];   // scale of a slot's value row over the cap
+      if constexpr (kQuantised<FMT>) {
+        float top = vs[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s) top = fmaxf(top, vs[s]);
+        if (__ballot(top > cap) != 0ull) {
+          top = max_over_quarters(top);
+          const uint32_t e = ((__builtin_bit_cast(uint32_t, top) + 0x7fffffu) & 0x7f800000u) + 0x800000u;   // twice the power of two at or above it
+          const float raised = __builtin_bit_cast(float, e < 0x7e000000u ? e : 0x7e000000u);
+          const float drop = cap / raised;
+          cap = raised;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[r][c] *= drop;
+        }
+        const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, cap));   // 1 / cap
+#pragma unroll
+        for (int s = 0; s < 8; ++s) weight[s] = vs[s] * unit;
+      }
+
+      // ---- weights.  A lane's sum that exceeds the headroom (an infinite one in the first tile) sends the tile through the
+      // pass that moves the references.
+      u32x4 pf[RT], pf_lo[RT];
+      float ps[RT][8], sum[RT], most = 0.0f;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        float xs[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          xs[s] = sc[r][s >> 2][s & 3] * (kQuantised<FMT> ? ks[s] : p.scale_log2e);
-          if (!ok[s]) xs[s] = -INFINITY;
+        for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][s >> 2][s & 3], kf[s], kWeightLog2<kPF16> - m_ref[r]));
+        sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
+        most = fmaxf(most, sum[r]);
+      }
+      if (__ballot(most > kMostWeight<kPF16>) != 0ull) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          float xs[8];
+#pragma unroll
+          for (int s = 0; s < 8; ++s) xs[s] = sc[r][s >> 2][s & 3] * kf[s];
+          float top = xs[0];
+#pragma unroll
+          for (int s = 1; s < 8; ++s) top = fmaxf(top, xs[s]);
+          const float m_new = fmaxf(m_ref[r], max_over_quarters(top));
+          const float alpha = __builtin_amdgcn_exp2f(m_ref[r] - m_new);
+          m_ref[r] = m_new;
+          l_run[r] *= alpha;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) acc[r][c] *= alpha;
+#pragma unroll
+          for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(xs[s] + (kWeightLog2<kPF16> - m_new));
+          sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
         }
-        float top = xs[0];
+      }
 #pragma unroll
-        for (int s = 1; s < 8; ++s) top = fmaxf(top, xs[s]);
-        top = max_over_quarters(top);
-        const float m_new = fmaxf(m_run[r], top);
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;   // nothing but masked rows so far
-        const float alpha = __builtin_amdgcn_exp2f(m_run[r] - m_use);
-        float ps[8], sum = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          ps[s] = __builtin_amdgcn_exp2f(xs[s] - (m_use - kWeightLog2<kPF16>));
-          sum += ps[s];
-        }
-        m_run[r] = m_new;
-        l_run[r] = l_run[r] * alpha + sum;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) acc[r][c] *= alpha;
+      for (int r = 0; r < RT; ++r) {
+        l_run[r] += sum[r];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float a = ps[2 * w], b = ps[2 * w + 1];
+          const float a = ps[r][2 * w], b = ps[r][2 * w + 1];
           if constexpr (kPF16) {
             const float x = kQuantised<FMT> ? a * weight[2 * w] : a, y = kQuantised<FMT> ? b * weight[2 * w + 1] : b;
             pf[r][w] = pack_f16(x, y);
@@ -331,36 +440,97 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
           }
         }
       }
-    }
 
-    const auto values = [&](auto d) {
-      constexpr int D = decltype(d)::value;
-      u32x4 even, odd;
-      v_frags<FMT, D>(vr, &even, &odd);
+      // ---- values
+      const auto values = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        u32x4 even, odd;
+        v_frags<FMT, D>(vr, &even, &odd);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        acc[r][2 * D] = mfma<kPF16>(even, pf[r], acc[r][2 * D]);
-        acc[r][2 * D + 1] = mfma<kPF16>(odd, pf[r], acc[r][2 * D + 1]);
-        if constexpr (kSplit) {
-          acc[r][2 * D] = mfma<kPF16>(even, pf_lo[r], acc[r][2 * D]);
-          acc[r][2 * D + 1] = mfma<kPF16>(odd, pf_lo[r], acc[r][2 * D + 1]);
+        for (int r = 0; r < RT; ++r) {
+          acc[r][2 * D] = mfma<kPF16>(even, pf[r], acc[r][2 * D]);
+          acc[r][2 * D + 1] = mfma<kPF16>(odd, pf[r], acc[r][2 * D + 1]);
+          if constexpr (kSplit) {
+            acc[r][2 * D] = mfma<kPF16>(even, pf_lo[r], acc[r][2 * D]);
+            acc[r][2 * D + 1] = mfma<kPF16>(odd, pf_lo[r], acc[r][2 * D + 1]);
+          }
         }
+      };
+      values(std::integral_constant<int, 0>());
+      values(std::integral_constant<int, 1>());
+      values(std::integral_constant<int, 2>());
+      values(std::integral_constant<int, 3>());
+      if (!more) break;
+      load_values(next);
+      tile = next_tile;
+      start = next;
+      rest -= WAVES * kTile;
+    }
+  };
+  if constexpr (INDEXED) {   // the ids of up to kStagedIds positions at a time, skipped ones as -1
+    for (int begin = it.begin, rest = it.end - it.begin; rest > 0; begin += kStagedIds, rest -= kStagedIds) {
+      const int count = min(rest, kStagedIds);
+      if (begin > it.begin) __syncthreads();
+      for (int i = tid; i < (count + kTile - 1) / kTile * kTile; i += WAVES * kWave) {
+        const int id = i < count ? it.idx[begin + i] : -1;
+        sh_ids[i] = id >= 0 && id < it.len ? id : -1;
       }
-    };
-    values(std::integral_constant<int, 0>());
-    values(std::integral_constant<int, 1>());
-    values(std::integral_constant<int, 2>());
-    values(std::integral_constant<int, 3>());
+      __syncthreads();
+      run(0, count);
+    }
+  } else {
+    run(it.begin, it.end);
   }
 
-  // ---- join the waves, sixteen query rows at a time
+  };   // attend_source
+  attend_source(item.first, wave);
+  if (item.two) {   // the waves that had one tile less go on
+    const int before = ((item.first.end - item.first.begin + kTile - 1) / kTile) % WAVES;
+    attend_source(item.second, wave >= before ? wave - before : wave - before + WAVES);
+  }
+
+  // ---- join the waves.  More than four: the upper four hand their state to the four below them, lane by lane.
+  if constexpr (WAVES > kJoined) {
+    static_assert(RT == 1 && WAVES % kJoined == 0, "");
+#pragma unroll
+    for (int from = WAVES - kJoined; from >= kJoined; from -= kJoined) {
+      const int slot = wave & (kJoined - 1);
+      if (from + kJoined < WAVES) __syncthreads();
+      if (wave >= from && wave < from + kJoined) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *(f32x4*)&sh.acc[slot][n][32 * j + 4 * c] = acc[0][c];
+        sh.state[slot][lane][0] = m_ref[0];
+        sh.state[slot][lane][1] = l_run[0];
+        sh.state[slot][lane][2] = cap;
+      }
+      __syncthreads();
+      if (wave >= from - kJoined && wave < from) {
+        const float m_other = sh.state[slot][lane][0], m = fmaxf(m_ref[0], m_other);
+        const float fa = __builtin_amdgcn_exp2f(m_ref[0] - m), fb = __builtin_amdgcn_exp2f(m_other - m);
+        l_run[0] = l_run[0] * fa + sh.state[slot][lane][1] * fb;
+        m_ref[0] = m;
+        float ga = fa, gb = fb;
+        if constexpr (kQuantised<FMT>) {
+          const float cap_other = sh.state[slot][lane][2], both = fmaxf(cap, cap_other);
+          ga *= cap / both;
+          gb *= cap_other / both;
+          cap = both;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[0][c] = acc[0][c] * ga + *(const f32x4*)&sh.acc[slot][n][32 * j + 4 * c] * gb;
+      }
+    }
+    __syncthreads();
+  }
+  // Sixteen query rows at a time, normalised.
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const float l = sum_over_quarters(l_run[r]);
     const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (kQuantised<FMT> ? cap : 1.0f);   // (an empty wave holds zeros)
     if (r) __syncthreads();
+    if (wave < kJoined) {
     if (j == 0) {
-      sh.m[wave][n] = m_run[r];
+      sh.m[wave][n] = m_ref[r];
       sh.l[wave][n] = l;
     }
 #pragma unroll
@@ -369,104 +539,127 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
       *(f32x4*)to = (f32x4){acc[r][0][i], acc[r][1][i], acc[r][2][i], acc[r][3][i]} * norm;
       *(f32x4*)(to + 4) = (f32x4){acc[r][4][i], acc[r][5][i], acc[r][6][i], acc[r][7][i]} * norm;
     }
+    }
     __syncthreads();
     // sixteen threads a row, eight dims each
-    const int row = it.row0 + 16 * r + (tid >> 4), d0 = 8 * (tid & 15);
-    if (row < it.row_end) {
-      float M = -INFINITY, w[kWaves], L = 0.0f;   // w: l 2^(m - M) of the waves
+    const int row = item.row0 + 16 * r + (tid >> 4), d0 = 8 * (tid & 15);
+    if (tid < 16 * 16 && row < item.row_end) {
+      float M = kNoReference, w[kJoined], L = 0.0f;   // w: l 2^(m - M) of the waves
 #pragma unroll
-      for (int x = 0; x < kWaves; ++x) M = fmaxf(M, sh.m[x][tid >> 4]);
-      const float m_use = M == -INFINITY ? 0.0f : M;
+      for (int x = 0; x < kJoined; ++x) M = fmaxf(M, sh.m[x][tid >> 4]);
       f32x4 lo = (f32x4){0.f, 0.f, 0.f, 0.f}, hi = lo;
 #pragma unroll
-      for (int x = 0; x < kWaves; ++x) {
-        w[x] = sh.l[x][tid >> 4] * __builtin_amdgcn_exp2f(sh.m[x][tid >> 4] - m_use);
+      for (int x = 0; x < kJoined; ++x) {
+        w[x] = sh.l[x][tid >> 4] * __builtin_amdgcn_exp2f(sh.m[x][tid >> 4] - M);   // (0 without rows)
         L += w[x];
       }
       const bool some = L > 0.0f || L != L;
       const float inv = some ? 1.0f / L : 0.0f;
 #pragma unroll
-      for (int x = 0; x < kWaves; ++x) {
+      for (int x = 0; x < kJoined; ++x) {
         lo += *(const f32x4*)&sh.acc[x][tid >> 4][d0] * (w[x] * inv);
         hi += *(const f32x4*)&sh.acc[x][tid >> 4][d0 + 4] * (w[x] * inv);
       }
-      const int b = it.b0 + (row >> p.group_log2), hq = it.h * group + (row & (group - 1));
+      const int b = item.b0 + (row >> p.group_log2), hq = item.h * group + (row & (group - 1));
       const int64_t flat = (int64_t)b * p.num_kv_heads * group + hq;
       if (p.num_splits > 1) {
-        const int64_t slot = flat * p.num_splits + it.slot;
+        const int64_t slot = flat * p.num_splits + item.slot;
         f32x4* to = (f32x4*)(p.part_acc + slot * kHeadDim + d0);
         to[0] = lo;
         to[1] = hi;
-        if (d0 == 0) {
-          p.part_m[slot] = M - kWeightLog2<kPF16>;   // (the sum as it is held belongs to a maximum that much lower)
-          p.part_l[slot] = L;
-        }
+        // (the sum as it is held belongs to a reference that much lower)
+        if (d0 == 0) p.part_ml[slot] = (f32x2){M == kNoReference ? M : M - kWeightLog2<kPF16>, L};
       } else {
-        u32x4 o;
-        if (p.out_dtype == TKA_F16) o = (u32x4){pack_f16(lo[0], lo[1]), pack_f16(lo[2], lo[3]), pack_f16(hi[0], hi[1]), pack_f16(hi[2], hi[3])};
-        else o = (u32x4){pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3])};
-        *(u32x4*)((uint16_t*)p.out + b * p.out_stride_b + (int64_t)hq * kHeadDim + d0) = o;
-        if (p.out_lse && d0 == 0) p.out_lse[flat] = some ? (M + (__builtin_log2f(L) - kWeightLog2<kPF16>)) * 0.69314718055994531f : -INFINITY;
+        store_row(p, b, hq, d0, lo, hi, M, L, kWeightLog2<kPF16>);
       }
     }
   }
 }
 
-__device__ __forceinline__ void point_at(const KvRows& rows, int b, int h, AttendItem* it) {
-  it->k = rows.k + b * rows.stride_b + h * rows.stride_h;
-  it->v = rows.v + b * rows.stride_b + h * rows.stride_h;
-  it->ks = rows.ks + b * rows.scale_b + h * rows.scale_h;
-  it->vs = rows.vs + b * rows.scale_b + h * rows.scale_h;
-  it->stride_n = rows.stride_n;
-  it->scale_n = rows.scale_n;
+__device__ __forceinline__ void point_at(const KvRows& rows, int b, int h, AttendSource* src) {
+  src->k = rows.k + b * rows.stride_b + h * rows.stride_h;
+  src->v = rows.v + b * rows.stride_b + h * rows.stride_h;
+  src->ks = rows.ks + b * rows.scale_b + h * rows.scale_h;
+  src->vs = rows.vs + b * rows.scale_b + h * rows.scale_h;
+  src->stride_n = rows.stride_n;
+  src->scale_n = rows.scale_n;
+  src->idx = nullptr;
+}
+
+__device__ __forceinline__ void take_shared(const KvAttendParams& p, int split, int h, AttendSource* src) {
+  point_at(p.shared, 0, h, src);
+  src->len = (int)p.shared.rows;
+  src->begin = split * p.shared_tps;   // (below the rows)
+  src->end = src->begin + min(src->len - src->begin, p.shared_tps);
+}
+
+template <bool INDEXED>
+__device__ __forceinline__ void take_own(const KvAttendParams& p, int split, int b, int h, AttendSource* src) {
+  point_at(p.own, b, h, src);
+  src->len = (int)p.own.rows;
+  if (p.own_len) src->len = __builtin_amdgcn_readfirstlane(max(min(p.own_len[b], src->len), 0));
+  int count = src->len;
+  if (INDEXED) {
+    const int64_t seg = (int64_t)b * p.num_kv_heads + h;
+    src->idx = p.kv_idx + seg * p.idx_len;
+    count = p.kv_count ? __builtin_amdgcn_readfirstlane(max(min(p.kv_count[seg], p.idx_len), 0)) : p.idx_len;
+  }
+  src->begin = split * p.own_tps;      // (below the capacity; the length may end before it)
+  src->end = src->begin + min(count - src->begin, p.own_tps);
 }
 
 // RT: sixteens of query rows that a workgroup of the shared source takes (0: there is no shared source)
 template <int DT, int FMT, int RT, bool INDEXED>
-__global__ __launch_bounds__(kThreads) void kv_attend_kernel(KvAttendParams p) {
+__global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_attend_kernel(KvAttendParams p) {
   __shared__ AttendLds sh;
+  __shared__ __align__(16) int32_t sh_ids[INDEXED ? kStagedIds : 4];
   const uint32_t shared_items = RT ? (uint32_t)(p.row_blocks * p.num_kv_heads * p.shared_splits) : 0u;
-  AttendItem it;
+  AttendItem item;
+  item.two = false;
   if (RT && blockIdx.x < shared_items) {
     const uint32_t split = blockIdx.x % (uint32_t)p.shared_splits, rest = blockIdx.x / (uint32_t)p.shared_splits;
-    it.h = (int)(rest % (uint32_t)p.num_kv_heads);
-    it.row0 = (int)(rest / (uint32_t)p.num_kv_heads) * 16 * RT;
-    it.row_end = p.batch << p.group_log2;
-    it.b0 = 0;
-    it.idx = nullptr;
-    it.len = p.shared.rows;
-    it.begin = (int64_t)split * p.shared_tps;
-    it.end = it.begin + p.shared_tps;
-    it.end = it.end < it.len ? it.end : it.len;
-    it.slot = (int)split;
-    point_at(p.shared, 0, it.h, &it);
-    attend<DT, FMT, RT ? RT : 1, false>(p, it, sh);
+    item.h = (int)(rest % (uint32_t)p.num_kv_heads);
+    item.row0 = (int)(rest / (uint32_t)p.num_kv_heads) * 16 * RT;
+    item.row_end = p.batch << p.group_log2;
+    item.b0 = 0;
+    item.slot = (int)split;
+    take_shared(p, (int)split, item.h, &item.first);
+    attend<DT, FMT, RT ? RT : 1, false, kWaves>(p, item, sh, sh_ids);
     return;
   }
-  const uint32_t item = blockIdx.x - shared_items;
-  const uint32_t split = item % (uint32_t)p.own_splits, seg = item / (uint32_t)p.own_splits;
-  it.b0 = (int)(seg / (uint32_t)p.num_kv_heads);
-  it.h = (int)(seg % (uint32_t)p.num_kv_heads);
-  it.row0 = 0;
-  it.row_end = 1 << p.group_log2;
-  it.len = p.own.rows;
-  if (p.own_len) {
-    const int64_t len = p.own_len[it.b0];
-    it.len = len < 0 ? 0 : (len < it.len ? len : it.len);
+  const uint32_t own = blockIdx.x - shared_items;
+  const uint32_t split = own % (uint32_t)p.own_splits, seg = own / (uint32_t)p.own_splits;
+  item.b0 = (int)(seg / (uint32_t)p.num_kv_heads);
+  item.h = (int)(seg % (uint32_t)p.num_kv_heads);
+  item.row0 = 0;
+  item.row_end = 1 << p.group_log2;
+  item.slot = p.shared_splits + (int)split;
+  take_own<INDEXED>(p, (int)split, item.b0, item.h, &item.first);
+  attend<DT, FMT, 1, INDEXED, kWaves>(p, item, sh, sh_ids);
+}
+
+// Short calls: one workgroup of eight waves per (entry, head) attends to everything and writes the result, one launch.  The
+// shared rows are then read for each entry.
+constexpr int kSoloWaves = 8;
+template <int DT, int FMT, bool SHARED, bool INDEXED>
+__global__ __launch_bounds__(kSoloWaves * kWave, 2) void kv_attend_solo_kernel(KvAttendParams p) {
+  __shared__ AttendLds sh;
+  __shared__ __align__(16) int32_t sh_ids[INDEXED ? kStagedIds : 4];
+  AttendItem item;
+  item.b0 = (int)(blockIdx.x / (uint32_t)p.num_kv_heads);
+  item.h = (int)(blockIdx.x % (uint32_t)p.num_kv_heads);
+  item.row0 = 0;
+  item.row_end = 1 << p.group_log2;
+  item.slot = 0;
+  item.two = false;
+  if constexpr (SHARED) {
+    take_shared(p, 0, item.h, &item.first);
+    item.two = p.own_splits != 0;
+    if (item.two) take_own<false>(p, 0, item.b0, item.h, &item.second);
+  } else {
+    take_own<INDEXED>(p, 0, item.b0, item.h, &item.first);
   }
-  int64_t count = it.len;
-  it.idx = nullptr;
-  if (INDEXED) {
-    it.idx = p.kv_idx + (int64_t)seg * p.idx_len;
-    count = p.kv_count ? p.kv_count[seg] : p.idx_len;
-    count = count < 0 ? 0 : (count < p.idx_len ? count : p.idx_len);
-  }
-  it.begin = (int64_t)split * p.own_tps;
-  it.end = it.begin + p.own_tps;
-  it.end = it.end < count ? it.end : count;
-  it.slot = p.shared_splits + (int)split;
-  point_at(p.own, it.b0, it.h, &it);
-  attend<DT, FMT, 1, INDEXED>(p, it, sh);
+  attend<DT, FMT, 1, INDEXED, kSoloWaves>(p, item, sh, sh_ids);
 }
 
 // One workgroup per query row: 32 lanes hold the 128 dims, eight groups of them take every eighth split.  A row whose sum is
@@ -476,16 +669,14 @@ __global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttendParams p) 
   __shared__ f32x4 sh_o[kCombineGroups][32];
   const int64_t row = blockIdx.x;
   const int g = threadIdx.x >> 5, d = threadIdx.x & 31, S = p.num_splits;
-  const float* pm = p.part_m + row * S;
-  const float* pl = p.part_l + row * S;
+  const f32x2* ml = p.part_ml + row * S;
   const f32x4* pa = (const f32x4*)(p.part_acc + row * S * kHeadDim) + d;
-  float M = -INFINITY;
-  for (int s = d; s < S; s += 32) M = fmaxf(M, pm[s]);   // (every group reads all maxima and sums: a line or two)
+  float M = kNoReference;
+  for (int s = d; s < S; s += 32) M = fmaxf(M, ml[s][0]);   // (every group reads all references and sums: a line or two)
 #pragma unroll
   for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-  const float m_use = M == -INFINITY ? 0.0f : M;
   float L = 0.0f;
-  for (int s = d; s < S; s += 32) L += pl[s] * __builtin_amdgcn_exp2f(pm[s] - m_use);
+  for (int s = d; s < S; s += 32) L += ml[s][1] * __builtin_amdgcn_exp2f(ml[s][0] - M);
 #pragma unroll
   for (int x = 16; x >= 1; x >>= 1) L += __shfl_xor(L, x, 64);
   const bool some = L > 0.0f || L != L;
@@ -498,7 +689,7 @@ __global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttendParams p) 
     for (int u = 0; u < 4; ++u) {
       const int s = s0 + u * kCombineGroups, sc = s < S ? s : s0;
       a[u] = pa[(int64_t)sc * 32];
-      w[u] = pl[sc] * __builtin_amdgcn_exp2f(pm[sc] - m_use) * inv;
+      w[u] = ml[sc][1] * __builtin_amdgcn_exp2f(ml[sc][0] - M) * inv;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -518,7 +709,24 @@ __global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttendParams p) 
 }
 
 template <int DT, int FMT>
-int launch_typed(const KvAttendParams& p, int row_tiles, uint32_t grid, hipStream_t stream) {
+int launch_solo(const KvAttendParams& p, hipStream_t stream) {
+  const uint32_t grid = (uint32_t)(p.batch * p.num_kv_heads);
+  constexpr int threads = kSoloWaves * kWave;
+  if (p.kv_idx) {
+    if constexpr (kQuantised<FMT>) kv_attend_solo_kernel<DT, FMT, false, true><<<grid, threads, 0, stream>>>(p);
+    else return TKA_EUNSUPPORTED;
+  } else if (p.shared_splits) {
+    kv_attend_solo_kernel<DT, FMT, true, false><<<grid, threads, 0, stream>>>(p);
+  } else {
+    kv_attend_solo_kernel<DT, FMT, false, false><<<grid, threads, 0, stream>>>(p);
+  }
+  return hip_status(hipGetLastError());
+}
+
+template <int DT, int FMT>
+int launch_typed(const KvAttendParams& p, int row_tiles, hipStream_t stream) {
+  if (row_tiles == 0) return launch_solo<DT, FMT>(p, stream);
+  const uint32_t grid = (uint32_t)(p.row_blocks * p.num_kv_heads * p.shared_splits + p.batch * p.num_kv_heads * p.own_splits);
   if (p.kv_idx) {
     if constexpr (kQuantised<FMT>) kv_attend_kernel<DT, FMT, 0, true><<<grid, kThreads, 0, stream>>>(p);
     else return TKA_EUNSUPPORTED;
@@ -535,21 +743,19 @@ int launch_typed(const KvAttendParams& p, int row_tiles, uint32_t grid, hipStrea
 }
 
 template <int DT>
-int launch_format(const KvAttendParams& p, int format, int row_tiles, uint32_t grid, hipStream_t stream) {
+int launch_format(const KvAttendParams& p, int format, int row_tiles, hipStream_t stream) {
   switch (format) {
-    case TKA_KV_16BIT: return launch_typed<DT, TKA_KV_16BIT>(p, row_tiles, grid, stream);
-    case TKA_KV_E4M3: return launch_typed<DT, TKA_KV_E4M3>(p, row_tiles, grid, stream);
-    default: return launch_typed<DT, TKA_KV_INT8>(p, row_tiles, grid, stream);
+    case TKA_KV_16BIT: return launch_typed<DT, TKA_KV_16BIT>(p, row_tiles, stream);
+    case TKA_KV_E4M3: return launch_typed<DT, TKA_KV_E4M3>(p, row_tiles, stream);
+    default: return launch_typed<DT, TKA_KV_INT8>(p, row_tiles, stream);
   }
 }
 
 }  // namespace
 
 int launch_kv_attend(const KvAttendParams& p, int dtype, int format, int row_tiles, hipStream_t stream) {
-  const uint32_t grid = (uint32_t)(p.row_blocks * p.num_kv_heads * p.shared_splits + p.batch * p.num_kv_heads * p.own_splits);
   LaunchTimer timer(p.shared_splits ? "prefix_attend" : (p.kv_idx ? "kvq_attend_indexed" : "kvq_attend_dense"), stream);
-  return dtype == TKA_F16 ? launch_format<TKA_F16>(p, format, row_tiles, grid, stream)
-                          : launch_format<TKA_BF16>(p, format, row_tiles, grid, stream);
+  return dtype == TKA_F16 ? launch_format<TKA_F16>(p, format, row_tiles, stream) : launch_format<TKA_BF16>(p, format, row_tiles, stream);
 }
 
 int launch_kv_combine(const KvAttendParams& p, hipStream_t stream) {

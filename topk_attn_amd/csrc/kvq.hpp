@@ -5,6 +5,8 @@
 
 namespace tka {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 // Strides of code rows are in BYTES, those of scales in elements; a stride of 0 shares the cache among the batch.
 struct KvRows {
   const unsigned char* k;
@@ -59,17 +61,18 @@ struct KvAttendParams {
   const int32_t* kv_count;  // [batch][num_kv_heads] or nullptr
   int idx_len;
   int num_splits;           // partials per query row: shared_splits + own_splits
-  float* part_m;            // [rows][num_splits], base-2 maxima
-  float* part_l;
-  float* part_acc;          // [rows][num_splits][128]
-  void* out;                // written here when num_splits == 1, else by the combine launch
+  f32x2* part_ml;           // [rows][num_splits] reference (base 2) and sum of the weights
+  float* part_acc;          // [rows][num_splits][128], normalised
+  void* out;
   float* out_lse;
   int64_t out_stride_b;
   int out_dtype;
   float scale_log2e;
 };
 constexpr int kAttendTile = 32;   // tokens of a wave's tile
+// row_tiles: RT of the shared source; 0 = the short form, one workgroup per (entry, head) and one split of each source.
 int launch_kv_attend(const KvAttendParams& p, int dtype, int format, int row_tiles, hipStream_t stream);
+
 // Joins the partials of the query rows and writes p.out / p.out_lse (num_splits > 1).
 int launch_kv_combine(const KvAttendParams& p, hipStream_t stream);
 
