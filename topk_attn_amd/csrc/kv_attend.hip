@@ -193,296 +193,369 @@ __device__ __forceinline__ void store_row(const KvAttendParams& p, int b, int hq
     p.out_lse[(((int64_t)b * p.num_kv_heads) << p.group_log2) + hq] = L > 0.0f || L != L ? (M + (__builtin_log2f(L) - l_log2)) * 0.69314718055994531f : -INFINITY;
 }
 
-template <int DT, int FMT, int RT, bool INDEXED, int WAVES>
-__device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem& item, AttendLds& sh, int32_t* sh_ids) {
-  constexpr bool kQF16 = DT == TKA_F16;
-  constexpr bool kPF16 = kQuantised<FMT> || DT == TKA_F16;   // type of the second product
-  constexpr bool kSplit = !kPF16 || DT == TKA_F16;           // weights in two parts
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, j = lane >> 4;
-  const int group = 1 << p.group_log2;
-
-  u32x4 qf[RT][4];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = item.row0 + 16 * r + n;
-    const bool there = row < item.row_end;
-    const int rr = there ? row : 0;
-    const uint16_t* q = (const uint16_t*)p.q + (int64_t)(item.b0 + (rr >> p.group_log2)) * p.q_stride_b +
-                        (int64_t)(item.h * group + (rr & (group - 1))) * kHeadDim;
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      qf[r][kb] = *(const u32x4*)(q + k_dim<FMT>(kb, j));
-      if (!there) qf[r][kb] = (u32x4){0u, 0u, 0u, 0u};
-    }
-  }
-
-  float m_ref[RT], l_run[RT];   // of query row n of each tile; l_run: this quarter's share
+// What a wave holds of its 16 RT query rows (row n of each sixteen in the lanes n, n + 16, n + 32, n + 48).
+template <int DT, int FMT, int RT>
+struct Rows {
+  static constexpr bool kQF16 = DT == TKA_F16;
+  static constexpr bool kPF16 = kQuantised<FMT> || DT == TKA_F16;   // type of the second product
+  static constexpr bool kSplit = !kPF16 || DT == TKA_F16;           // weights in two parts
+  u32x4 q[RT][4];
+  float m_ref[RT], l_run[RT];   // l_run: this quarter's share
   f32x4 acc[RT][8];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    m_ref[r] = kNoReference;
-    l_run[r] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) acc[r][c] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  }
-  float cap = __builtin_bit_cast(float, 17u << 23);   // 2^-110: the least cap (its reciprocal stays in range)
+  float cap;
 
-  // One source: its tiles go round the waves, `turn` is this wave's first.
-  const auto attend_source = [&](const AttendSource& it, int turn) {
-  KTile<FMT> kt[2];
-  VRow<FMT> vr[8];
-  float ks[8], vs[8];
-  // Rows of a tile of 32 positions from `start`: key rows 16x + n, value and scale rows the slot tokens.  Dense: a scalar
-  // base and 32-bit lane offsets (32 strides fit, the host checks), rows that a source of less than 32 does not have
-  // replaced by its last.  Listed: the ids of the positions, -1 replaced by row 0.
+  // Rows [row0, row0 + 16 RT) below row_end; row r is head h * group + r % group of entry b0 + r / group.
+  __device__ __forceinline__ void begin(const KvAttendParams& p, int b0, int h, int row0, int row_end) {
+    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4, group = 1 << p.group_log2;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = row0 + 16 * r + n;
+      const bool there = row < row_end;
+      const int rr = there ? row : 0;
+      const uint16_t* of = (const uint16_t*)p.q + (int64_t)(b0 + (rr >> p.group_log2)) * p.q_stride_b +
+                           (int64_t)(h * group + (rr & (group - 1))) * kHeadDim;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        q[r][kb] = *(const u32x4*)(of + k_dim<FMT>(kb, j));
+        if (!there) q[r][kb] = (u32x4){0u, 0u, 0u, 0u};
+      }
+      m_ref[r] = kNoReference;
+      l_run[r] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[r][c] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    cap = __builtin_bit_cast(float, 17u << 23);   // 2^-110: the least cap (its reciprocal stays in range)
+  }
+
+  // Logits of a tile of 32 tokens, before their factors.  key_frag(x, kb): operand of sixteen x and k-block kb.
+  template <typename KeyFrag>
+  __device__ __forceinline__ void scores(f32x4 (&sc)[RT][2], KeyFrag key_frag) const {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) sc[r][0] = sc[r][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        const u32x4 a = key_frag(x, kb);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) sc[r][x] = mfma<kQF16>(a, q[r][kb], sc[r][x]);
+      }
+  }
+
+  // The rest of it.  kf: factors of the slot tokens' logits, vs: their value scales; masked: bit s = slot s has no row
+  // (any_masked: some lane has one); value_frags(D, even, odd): operands of output dims 2 D and 2 D + 1.
+  // beside(): work that has nothing to do with this tile, beside its exponentials.
+  template <typename ValueFrags, typename Beside>
+  __device__ __forceinline__ void attend(f32x4 (&sc)[RT][2], float (&kf)[8], float (&vs)[8], uint32_t masked, bool any_masked, ValueFrags value_frags,
+                                         Beside beside) {
+    // masked slots have no weight (and their value rows are zeros: no 0 * inf, no 0 * NaN)
+    if (any_masked) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (masked >> s & 1u) {
+          vs[s] = 0.0f;
+          kf[s] = 1.0f;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) sc[r][s >> 2][s & 3] = -INFINITY;
+        }
+    }
+    float weight[8];   // scale of a slot's value row over the cap
+    if constexpr (kQuantised<FMT>) {
+      float top = fabsf(vs[0]);
+#pragma unroll
+      for (int s = 1; s < 8; ++s) top = fmaxf(top, fabsf(vs[s]));
+      if (__ballot(top > cap) != 0ull) {
+        top = max_over_quarters(top);
+        const uint32_t e = ((__builtin_bit_cast(uint32_t, top) + 0x7fffffu) & 0x7f800000u) + 0x800000u;   // twice the power of two at or above it
+        const float raised = __builtin_bit_cast(float, e < 0x7e000000u ? e : 0x7e000000u);
+        const float drop = cap / raised;
+        cap = raised;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) acc[r][c] *= drop;
+      }
+      const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, cap));   // 1 / cap
+#pragma unroll
+      for (int s = 0; s < 8; ++s) weight[s] = vs[s] * unit;
+    }
+
+    // ---- weights.  A lane's sum that exceeds the headroom (an infinite one in the first tile) sends the tile through the
+    // pass that moves the references.
+    u32x4 pf[RT], pf_lo[RT];
+    float ps[RT][8], sum[RT], most = 0.0f;
+    beside();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][s >> 2][s & 3], kf[s], kWeightLog2<kPF16> - m_ref[r]));
+      sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
+      most = fmaxf(most, sum[r]);
+    }
+    if (__ballot(most > kMostWeight<kPF16>) != 0ull) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float xs[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) xs[s] = sc[r][s >> 2][s & 3] * kf[s];
+        float top = xs[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s) top = fmaxf(top, xs[s]);
+        const float m_new = fmaxf(m_ref[r], max_over_quarters(top));
+        const float alpha = __builtin_amdgcn_exp2f(m_ref[r] - m_new);
+        m_ref[r] = m_new;
+        l_run[r] *= alpha;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[r][c] *= alpha;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(xs[s] + (kWeightLog2<kPF16> - m_new));
+        sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      l_run[r] += sum[r];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float a = ps[r][2 * w], b = ps[r][2 * w + 1];
+        if constexpr (kPF16) {
+          const float x = kQuantised<FMT> ? a * weight[2 * w] : a, y = kQuantised<FMT> ? b * weight[2 * w + 1] : b;
+          pf[r][w] = pack_f16(x, y);
+          if constexpr (kSplit) {
+            uint32_t hi = pf[r][w];
+            asm("" : "+v"(hi));   // (the compiler otherwise folds the conversions into mixed-precision multiply-adds and takes the first pair's rounded weights for all four)
+            const f16x2 h = __builtin_bit_cast(f16x2, hi);
+            pf_lo[r][w] = pack_f16(x - (float)h[0], y - (float)h[1]);
+          }
+        } else {
+          pf[r][w] = pack_bf16(a, b);
+          pf_lo[r][w] = pack_bf16(a - __builtin_bit_cast(float, pf[r][w] << 16), b - __builtin_bit_cast(float, pf[r][w] & 0xffff0000u));
+        }
+      }
+    }
+
+    // ---- values
+    const auto values = [&](auto d) {
+      constexpr int D = decltype(d)::value;
+      u32x4 even, odd;
+      value_frags(d, &even, &odd);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        acc[r][2 * D] = mfma<kPF16>(even, pf[r], acc[r][2 * D]);
+        acc[r][2 * D + 1] = mfma<kPF16>(odd, pf[r], acc[r][2 * D + 1]);
+        if constexpr (kSplit) {
+          acc[r][2 * D] = mfma<kPF16>(even, pf_lo[r], acc[r][2 * D]);
+          acc[r][2 * D + 1] = mfma<kPF16>(odd, pf_lo[r], acc[r][2 * D + 1]);
+        }
+      }
+    };
+    values(std::integral_constant<int, 0>());
+    values(std::integral_constant<int, 1>());
+    values(std::integral_constant<int, 2>());
+    values(std::integral_constant<int, 3>());
+  }
+};
+
+// Rows of a dense source, a tile of 32 positions from `start`: key rows 16x + n, value and scale rows the slot tokens.  A scalar
+// base and 32-bit lane offsets (32 strides fit, the host checks); rows that a source of less than 32 does not have are
+// replaced by its last.
+template <int FMT>
+struct DenseTiles {
   uint32_t k_off[2], v_off[8];
-  const bool vector_scales = it.scale_n == 1 && it.end >= kTile;
-  if constexpr (!INDEXED) {
+  int last;
+  bool vector_scales;
+
+  __device__ __forceinline__ void begin(const AttendSource& it) {
+    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const uint32_t stride = (uint32_t)it.stride_n;
-    const int last = min(it.end, kTile) - 1;
+    last = min(it.end, kTile) - 1;
+    vector_scales = it.scale_n == 1 && it.end >= kTile;
 #pragma unroll
     for (int x = 0; x < 2; ++x) k_off[x] = (uint32_t)min(16 * x + n, last) * stride + 16u * j;
 #pragma unroll
     for (int s = 0; s < 8; ++s) v_off[s] = (uint32_t)min(slot_token(j, s), last) * stride + (kQuantised<FMT> ? 8u : 16u) * n;
   }
-  const auto load_scales = [&](const float* of_source, int start, float (&f)[8]) {
-    if constexpr (INDEXED) {
+  __device__ __forceinline__ void scales(const AttendSource& it, const float* of_source, int start, float (&f)[8]) const {
+    const int j = (threadIdx.x & 63) >> 4;
+    const float* base = of_source + (int64_t)start * it.scale_n;
+    if (vector_scales) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const f32x4u v = *(const f32x4u*)(base + 16 * x + 4u * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 * x + i] = v[i];
+      }
+    } else {
+      int most = last;
+      asm("" : "+s"(most));   // (the eight offsets are made here, not kept in registers over the loop)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) f[s] = *(const float*)((const unsigned char*)base + (uint32_t)min(slot_token(j, s), most) * (uint32_t)(4 * it.scale_n));
+    }
+  }
+  __device__ __forceinline__ void keys(const AttendSource& it, int start, KTile<FMT> (&kt)[2], float (&ks)[8]) const {
+    key_rows(it, start, kt);
+    if constexpr (kQuantised<FMT>) scales(it, it.ks, start, ks);
+  }
+  __device__ __forceinline__ void values(const AttendSource& it, int start, VRow<FMT> (&vr)[8], float (&vs)[8]) const {
+    value_rows(it, start, vr);
+    if constexpr (kQuantised<FMT>) scales(it, it.vs, start, vs);
+  }
+  __device__ __forceinline__ void key_rows(const AttendSource& it, int start, KTile<FMT> (&kt)[2]) const {
+    const unsigned char* base = it.k + (int64_t)start * it.stride_n;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(base + k_off[x] + 64 * y);
+  }
+  __device__ __forceinline__ void value_rows(const AttendSource& it, int start, VRow<FMT> (&vr)[8]) const {
+    const unsigned char* base = it.v + (int64_t)start * it.stride_n;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) vr[s] = *(const VRow<FMT>*)(base + v_off[s]);
+  }
+};
+
+// A dense tile that the end cuts starts earlier, at the last 32 rows that there are, and its first positions are masked.
+__device__ __forceinline__ int tile_start(int tile, int end) { return end - tile >= kTile ? tile : max(end - kTile, 0); }
+__device__ __forceinline__ uint32_t tile_mask(int start, int tile, int end) {
+  const int j = (threadIdx.x & 63) >> 4;
+  uint32_t masked = 0;
+#pragma unroll
+  for (int s = 0; s < 8; ++s) masked |= start + slot_token(j, s) < tile || start + slot_token(j, s) >= end ? 1u << s : 0u;
+  return masked;
+}
+template <int FMT>
+__device__ __forceinline__ void clear_masked(uint32_t masked, VRow<FMT> (&vr)[8]) {
+#pragma unroll
+  for (int s = 0; s < 8; ++s)
+    if (masked >> s & 1u) vr[s] = VRow<FMT>{};
+}
+
+// Partial of one split (a join follows) or the finished row, dims d0 .. d0 + 7.
+template <bool F16>
+__device__ __forceinline__ void store_result(const KvAttendParams& p, int b, int hq, int slot, int d0, const f32x4& lo, const f32x4& hi, float M, float L) {
+  if (p.num_splits > 1) {
+    const int64_t at = ((((int64_t)b * p.num_kv_heads) << p.group_log2) + hq) * p.num_splits + slot;
+    f32x4* to = (f32x4*)(p.part_acc + at * kHeadDim + d0);
+    to[0] = lo;
+    to[1] = hi;
+    // (the sum as it is held belongs to a reference that much lower)
+    if (d0 == 0) p.part_ml[at] = (f32x2){M == kNoReference ? M : M - kWeightLog2<F16>, L};
+  } else {
+    store_row(p, b, hq, d0, lo, hi, M, L, kWeightLog2<F16>);
+  }
+}
+
+template <int DT, int FMT, int RT, bool INDEXED, int WAVES>
+__device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem& item, AttendLds& sh, int32_t* sh_ids) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, j = lane >> 4;
+  const int group = 1 << p.group_log2;
+  Rows<DT, FMT, RT> rows;
+  rows.begin(p, item.b0, item.h, item.row0, item.row_end);
+
+  // One source: its tiles go round the waves, `turn` is this wave's first.  The keys of the next tile are asked for as soon as
+  // those of this one are in the matrix cores, its values behind this tile's.
+  const auto attend_source = [&](const AttendSource& it, int turn) {
+    KTile<FMT> kt[2];
+    VRow<FMT> vr[8];
+    float ks[8], vs[8];
+    DenseTiles<FMT> dense;
+    if constexpr (!INDEXED) dense.begin(it);
+    // Listed: rows by the ids of the positions in LDS, -1 replaced by row 0.
+    const auto listed_scales = [&](const float* of_source, int start, float (&f)[8]) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[4 * x + i] = of_source[(int64_t)max(id[i], 0) * it.scale_n];
       }
-    } else {
-      const float* base = of_source + (int64_t)start * it.scale_n;
-      if (vector_scales) {
+    };
+    const auto load_keys = [&](int start) {
+      if constexpr (INDEXED) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const f32x4u v = *(const f32x4u*)(base + 16 * x + 4u * j);
+          const unsigned char* row = it.k + (int64_t)max(sh_ids[start + 16 * x + n], 0) * it.stride_n + 16 * j;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f[4 * x + i] = v[i];
+          for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(row + 64 * y);
         }
+        listed_scales(it.ks, start, ks);
       } else {
-        int last = min(it.end, kTile) - 1;
-        asm("" : "+s"(last));   // (the eight offsets are made here, not kept in registers over the loop)
-#pragma unroll
-        for (int s = 0; s < 8; ++s) f[s] = *(const float*)((const unsigned char*)base + (uint32_t)min(slot_token(j, s), last) * (uint32_t)(4 * it.scale_n));
+        dense.keys(it, start, kt, ks);
       }
-    }
-  };
-  const auto load_keys = [&](int start) {
-    if constexpr (INDEXED) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const unsigned char* row = it.k + (int64_t)max(sh_ids[start + 16 * x + n], 0) * it.stride_n + 16 * j;
-#pragma unroll
-        for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(row + 64 * y);
-      }
-    } else {
-      const unsigned char* base = it.k + (int64_t)start * it.stride_n;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(base + k_off[x] + 64 * y);
-    }
-    if constexpr (kQuantised<FMT>) load_scales(it.ks, start, ks);
-  };
-  const auto load_values = [&](int start) {
-    if constexpr (INDEXED) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vr[4 * x + i] = *(const VRow<FMT>*)(it.v + (int64_t)max(id[i], 0) * it.stride_n + (kQuantised<FMT> ? 8 : 16) * n);
-      }
-    } else {
-      const unsigned char* base = it.v + (int64_t)start * it.stride_n;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) vr[s] = *(const VRow<FMT>*)(base + v_off[s]);
-    }
-    if constexpr (kQuantised<FMT>) load_scales(it.vs, start, vs);
-  };
-
-  // Positions [begin, end): the waves take tiles in turn.  The keys of the next tile are asked for as soon as those of this
-  // one are in the matrix cores, its values behind this tile's.  A dense tile that the end cuts starts earlier, at the last
-  // 32 rows that there are, and its first positions are masked (listed positions are filled up with -1).
-  const auto run = [&](int begin, int end) {
-    int rest = end - begin - turn * kTile;   // positions from this tile's first on
-    if (rest <= 0) return;
-    int tile = begin + turn * kTile;
-    int start = INDEXED || rest >= kTile ? tile : max(end - kTile, 0);
-    load_keys(start);
-    load_values(start);
-    while (true) {
-      asm("" : "+s"(start));   // (addresses are made from it in scalar registers, not carried along in vector registers)
-      const bool more = rest > WAVES * kTile;
-      const int next_tile = tile + WAVES * kTile;
-      const int next = INDEXED || rest >= (WAVES + 1) * kTile ? next_tile : max(end - kTile, 0);
-      uint32_t masked = 0;   // bit s: slot s has no row
-      bool any_masked;
+    };
+    const auto load_values = [&](int start) {
       if constexpr (INDEXED) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) masked |= id[i] < 0 ? 1u << (4 * x + i) : 0u;
+          for (int i = 0; i < 4; ++i) vr[4 * x + i] = *(const VRow<FMT>*)(it.v + (int64_t)max(id[i], 0) * it.stride_n + (kQuantised<FMT> ? 8 : 16) * n);
         }
-        any_masked = __ballot(masked != 0) != 0ull;
+        listed_scales(it.vs, start, vs);
       } else {
-        any_masked = rest < kTile;
-        if (any_masked) {
-#pragma unroll
-          for (int s = 0; s < 8; ++s) masked |= start + slot_token(j, s) < tile || start + slot_token(j, s) >= end ? 1u << s : 0u;
-        }
+        dense.values(it, start, vr, vs);
       }
+    };
 
-      // ---- logits, before their scales
-      f32x4 sc[RT][2];
+    // Positions [begin, end) (listed ones are filled up to whole tiles with -1).
+    const auto run = [&](int begin, int end) {
+      int rest = end - begin - turn * kTile;   // positions from this tile's first on
+      if (rest <= 0) return;
+      int tile = begin + turn * kTile;
+      int start = INDEXED ? tile : tile_start(tile, end);
+      load_keys(start);
+      load_values(start);
+      while (true) {
+        asm("" : "+s"(start));   // (addresses are made from it in scalar registers, not carried along in vector registers)
+        const bool more = rest > WAVES * kTile;
+        const int next_tile = tile + WAVES * kTile;
+        const int next = INDEXED || rest >= (WAVES + 1) * kTile ? next_tile : max(end - kTile, 0);
+        uint32_t masked = 0;
+        bool any_masked;
+        if constexpr (INDEXED) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r) sc[r][0] = sc[r][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          for (int x = 0; x < 2; ++x) {
+            const i32x4 id = *(const i32x4*)&sh_ids[start + 16 * x + 4 * j];
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          const u32x4 a = k_frag<FMT, kQF16>(kt[x], kb);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) sc[r][x] = mfma<kQF16>(a, qf[r][kb], sc[r][x]);
-        }
-      float kf[8];
-#pragma unroll
-      for (int s = 0; s < 8; ++s) kf[s] = kQuantised<FMT> ? ks[s] * p.scale_log2e : p.scale_log2e;
-      if (more) load_keys(next);
-
-      // masked slots: no weight, and nothing of their rows in the products (0 * inf, 0 * NaN)
-      if (any_masked) {
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          if (masked >> s & 1u) {
-            vr[s] = VRow<FMT>{};
-            vs[s] = 0.0f;
-            kf[s] = 1.0f;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) sc[r][s >> 2][s & 3] = -INFINITY;
+            for (int i = 0; i < 4; ++i) masked |= id[i] < 0 ? 1u << (4 * x + i) : 0u;
           }
-      }
-      float weight[8];   // scale of a slot's value row over the cap
-      if constexpr (kQuantised<FMT>) {
-        float top = vs[0];
-#pragma unroll
-        for (int s = 1; s < 8; ++s) top = fmaxf(top, vs[s]);
-        if (__ballot(top > cap) != 0ull) {
-          top = max_over_quarters(top);
-          const uint32_t e = ((__builtin_bit_cast(uint32_t, top) + 0x7fffffu) & 0x7f800000u) + 0x800000u;   // twice the power of two at or above it
-          const float raised = __builtin_bit_cast(float, e < 0x7e000000u ? e : 0x7e000000u);
-          const float drop = cap / raised;
-          cap = raised;
-#pragma unroll
-          for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int c = 0; c < 8; ++c) acc[r][c] *= drop;
+          any_masked = __ballot(masked != 0) != 0ull;
+        } else {
+          any_masked = rest < kTile;
+          if (any_masked) masked = tile_mask(start, tile, end);
         }
-        const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, cap));   // 1 / cap
+        float kf[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) weight[s] = vs[s] * unit;
+        for (int s = 0; s < 8; ++s) kf[s] = kQuantised<FMT> ? ks[s] * p.scale_log2e : p.scale_log2e;
+        f32x4 sc[RT][2];
+        rows.scores(sc, [&](int x, int kb) { return k_frag<FMT, Rows<DT, FMT, RT>::kQF16>(kt[x], kb); });
+        if (more) load_keys(next);
+        if (any_masked) clear_masked<FMT>(masked, vr);
+        rows.attend(sc, kf, vs, masked, any_masked, [&](auto d, u32x4* even, u32x4* odd) { v_frags<FMT, decltype(d)::value>(vr, even, odd); }, [] {});
+        if (!more) break;
+        load_values(next);
+        tile = next_tile;
+        start = next;
+        rest -= WAVES * kTile;
       }
-
-      // ---- weights.  A lane's sum that exceeds the headroom (an infinite one in the first tile) sends the tile through the
-      // pass that moves the references.
-      u32x4 pf[RT], pf_lo[RT];
-      float ps[RT][8], sum[RT], most = 0.0f;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-#pragma unroll
-        for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][s >> 2][s & 3], kf[s], kWeightLog2<kPF16> - m_ref[r]));
-        sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
-        most = fmaxf(most, sum[r]);
-      }
-      if (__ballot(most > kMostWeight<kPF16>) != 0ull) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          float xs[8];
-#pragma unroll
-          for (int s = 0; s < 8; ++s) xs[s] = sc[r][s >> 2][s & 3] * kf[s];
-          float top = xs[0];
-#pragma unroll
-          for (int s = 1; s < 8; ++s) top = fmaxf(top, xs[s]);
-          const float m_new = fmaxf(m_ref[r], max_over_quarters(top));
-          const float alpha = __builtin_amdgcn_exp2f(m_ref[r] - m_new);
-          m_ref[r] = m_new;
-          l_run[r] *= alpha;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) acc[r][c] *= alpha;
-#pragma unroll
-          for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(xs[s] + (kWeightLog2<kPF16> - m_new));
-          sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
+    };
+    if constexpr (INDEXED) {   // the ids of up to kStagedIds positions at a time, skipped ones as -1
+      for (int begin = it.begin, rest = it.end - it.begin; rest > 0; begin += kStagedIds, rest -= kStagedIds) {
+        const int count = min(rest, kStagedIds);
+        if (begin > it.begin) __syncthreads();
+        for (int i = tid; i < (count + kTile - 1) / kTile * kTile; i += WAVES * kWave) {
+          const int id = i < count ? it.idx[begin + i] : -1;
+          sh_ids[i] = id >= 0 && id < it.len ? id : -1;
         }
+        __syncthreads();
+        run(0, count);
       }
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        l_run[r] += sum[r];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float a = ps[r][2 * w], b = ps[r][2 * w + 1];
-          if constexpr (kPF16) {
-            const float x = kQuantised<FMT> ? a * weight[2 * w] : a, y = kQuantised<FMT> ? b * weight[2 * w + 1] : b;
-            pf[r][w] = pack_f16(x, y);
-            if constexpr (kSplit) {
-              uint32_t hi = pf[r][w];
-              asm("" : "+v"(hi));   // (the compiler otherwise folds the conversions into mixed-precision multiply-adds and takes the first pair's rounded weights for all four)
-              const f16x2 h = __builtin_bit_cast(f16x2, hi);
-              pf_lo[r][w] = pack_f16(x - (float)h[0], y - (float)h[1]);
-            }
-          } else {
-            pf[r][w] = pack_bf16(a, b);
-            pf_lo[r][w] = pack_bf16(a - __builtin_bit_cast(float, pf[r][w] << 16), b - __builtin_bit_cast(float, pf[r][w] & 0xffff0000u));
-          }
-        }
-      }
-
-      // ---- values
-      const auto values = [&](auto d) {
-        constexpr int D = decltype(d)::value;
-        u32x4 even, odd;
-        v_frags<FMT, D>(vr, &even, &odd);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          acc[r][2 * D] = mfma<kPF16>(even, pf[r], acc[r][2 * D]);
-          acc[r][2 * D + 1] = mfma<kPF16>(odd, pf[r], acc[r][2 * D + 1]);
-          if constexpr (kSplit) {
-            acc[r][2 * D] = mfma<kPF16>(even, pf_lo[r], acc[r][2 * D]);
-            acc[r][2 * D + 1] = mfma<kPF16>(odd, pf_lo[r], acc[r][2 * D + 1]);
-          }
-        }
-      };
-      values(std::integral_constant<int, 0>());
-      values(std::integral_constant<int, 1>());
-      values(std::integral_constant<int, 2>());
-      values(std::integral_constant<int, 3>());
-      if (!more) break;
-      load_values(next);
-      tile = next_tile;
-      start = next;
-      rest -= WAVES * kTile;
+    } else {
+      run(it.begin, it.end);
     }
+
   };
-  if constexpr (INDEXED) {   // the ids of up to kStagedIds positions at a time, skipped ones as -1
-    for (int begin = it.begin, rest = it.end - it.begin; rest > 0; begin += kStagedIds, rest -= kStagedIds) {
-      const int count = min(rest, kStagedIds);
-      if (begin > it.begin) __syncthreads();
-      for (int i = tid; i < (count + kTile - 1) / kTile * kTile; i += WAVES * kWave) {
-        const int id = i < count ? it.idx[begin + i] : -1;
-        sh_ids[i] = id >= 0 && id < it.len ? id : -1;
-      }
-      __syncthreads();
-      run(0, count);
-    }
-  } else {
-    run(it.begin, it.end);
-  }
-
-  };   // attend_source
   attend_source(item.first, wave);
   if (item.two) {   // the waves that had one tile less go on
     const int before = ((item.first.end - item.first.begin + kTile - 1) / kTile) % WAVES;
@@ -498,26 +571,26 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
       if (from + kJoined < WAVES) __syncthreads();
       if (wave >= from && wave < from + kJoined) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) *(f32x4*)&sh.acc[slot][n][32 * j + 4 * c] = acc[0][c];
-        sh.state[slot][lane][0] = m_ref[0];
-        sh.state[slot][lane][1] = l_run[0];
-        sh.state[slot][lane][2] = cap;
+        for (int c = 0; c < 8; ++c) *(f32x4*)&sh.acc[slot][n][32 * j + 4 * c] = rows.acc[0][c];
+        sh.state[slot][lane][0] = rows.m_ref[0];
+        sh.state[slot][lane][1] = rows.l_run[0];
+        sh.state[slot][lane][2] = rows.cap;
       }
       __syncthreads();
       if (wave >= from - kJoined && wave < from) {
-        const float m_other = sh.state[slot][lane][0], m = fmaxf(m_ref[0], m_other);
-        const float fa = __builtin_amdgcn_exp2f(m_ref[0] - m), fb = __builtin_amdgcn_exp2f(m_other - m);
-        l_run[0] = l_run[0] * fa + sh.state[slot][lane][1] * fb;
-        m_ref[0] = m;
+        const float m_other = sh.state[slot][lane][0], m = fmaxf(rows.m_ref[0], m_other);
+        const float fa = __builtin_amdgcn_exp2f(rows.m_ref[0] - m), fb = __builtin_amdgcn_exp2f(m_other - m);
+        rows.l_run[0] = rows.l_run[0] * fa + sh.state[slot][lane][1] * fb;
+        rows.m_ref[0] = m;
         float ga = fa, gb = fb;
         if constexpr (kQuantised<FMT>) {
-          const float cap_other = sh.state[slot][lane][2], both = fmaxf(cap, cap_other);
-          ga *= cap / both;
+          const float cap_other = sh.state[slot][lane][2], both = fmaxf(rows.cap, cap_other);
+          ga *= rows.cap / both;
           gb *= cap_other / both;
-          cap = both;
+          rows.cap = both;
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) acc[0][c] = acc[0][c] * ga + *(const f32x4*)&sh.acc[slot][n][32 * j + 4 * c] * gb;
+        for (int c = 0; c < 8; ++c) rows.acc[0][c] = rows.acc[0][c] * ga + *(const f32x4*)&sh.acc[slot][n][32 * j + 4 * c] * gb;
       }
     }
     __syncthreads();
@@ -525,19 +598,19 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
   // Sixteen query rows at a time, normalised.
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const float l = sum_over_quarters(l_run[r]);
-    const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (kQuantised<FMT> ? cap : 1.0f);   // (an empty wave holds zeros)
+    const float l = sum_over_quarters(rows.l_run[r]);
+    const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (kQuantised<FMT> ? rows.cap : 1.0f);   // (an empty wave holds zeros)
     if (r) __syncthreads();
     if (wave < kJoined) {
     if (j == 0) {
-      sh.m[wave][n] = m_ref[r];
+      sh.m[wave][n] = rows.m_ref[r];
       sh.l[wave][n] = l;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float* to = &sh.acc[wave][n][32 * j + 8 * i];
-      *(f32x4*)to = (f32x4){acc[r][0][i], acc[r][1][i], acc[r][2][i], acc[r][3][i]} * norm;
-      *(f32x4*)(to + 4) = (f32x4){acc[r][4][i], acc[r][5][i], acc[r][6][i], acc[r][7][i]} * norm;
+      *(f32x4*)to = (f32x4){rows.acc[r][0][i], rows.acc[r][1][i], rows.acc[r][2][i], rows.acc[r][3][i]} * norm;
+      *(f32x4*)(to + 4) = (f32x4){rows.acc[r][4][i], rows.acc[r][5][i], rows.acc[r][6][i], rows.acc[r][7][i]} * norm;
     }
     }
     __syncthreads();
@@ -560,18 +633,7 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
         lo += *(const f32x4*)&sh.acc[x][tid >> 4][d0] * (w[x] * inv);
         hi += *(const f32x4*)&sh.acc[x][tid >> 4][d0 + 4] * (w[x] * inv);
       }
-      const int b = item.b0 + (row >> p.group_log2), hq = item.h * group + (row & (group - 1));
-      const int64_t flat = (int64_t)b * p.num_kv_heads * group + hq;
-      if (p.num_splits > 1) {
-        const int64_t slot = flat * p.num_splits + item.slot;
-        f32x4* to = (f32x4*)(p.part_acc + slot * kHeadDim + d0);
-        to[0] = lo;
-        to[1] = hi;
-        // (the sum as it is held belongs to a reference that much lower)
-        if (d0 == 0) p.part_ml[slot] = (f32x2){M == kNoReference ? M : M - kWeightLog2<kPF16>, L};
-      } else {
-        store_row(p, b, hq, d0, lo, hi, M, L, kWeightLog2<kPF16>);
-      }
+      store_result<Rows<DT, FMT, RT>::kPF16>(p, item.b0 + (row >> p.group_log2), item.h * group + (row & (group - 1)), item.slot, d0, lo, hi, M, L);
     }
   }
 }
@@ -608,6 +670,21 @@ __device__ __forceinline__ void take_own(const KvAttendParams& p, int split, int
   src->end = src->begin + min(count - src->begin, p.own_tps);
 }
 
+// The own items of a launch: splits of (entry, head) pairs.
+template <int DT, int FMT, bool INDEXED>
+__device__ __forceinline__ void attend_own(const KvAttendParams& p, uint32_t own, AttendLds& sh, int32_t* sh_ids) {
+  const uint32_t split = own % (uint32_t)p.own_splits, seg = own / (uint32_t)p.own_splits;
+  AttendItem item;
+  item.two = false;
+  item.b0 = (int)(seg / (uint32_t)p.num_kv_heads);
+  item.h = (int)(seg % (uint32_t)p.num_kv_heads);
+  item.row0 = 0;
+  item.row_end = 1 << p.group_log2;
+  item.slot = p.shared_splits + (int)split;
+  take_own<INDEXED>(p, (int)split, item.b0, item.h, &item.first);
+  attend<DT, FMT, 1, INDEXED, kWaves>(p, item, sh, sh_ids);
+}
+
 // RT: sixteens of query rows that a workgroup of the shared source takes (0: there is no shared source)
 template <int DT, int FMT, int RT, bool INDEXED>
 __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_attend_kernel(KvAttendParams p) {
@@ -627,15 +704,137 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
     attend<DT, FMT, RT ? RT : 1, false, kWaves>(p, item, sh, sh_ids);
     return;
   }
-  const uint32_t own = blockIdx.x - shared_items;
-  const uint32_t split = own % (uint32_t)p.own_splits, seg = own / (uint32_t)p.own_splits;
-  item.b0 = (int)(seg / (uint32_t)p.num_kv_heads);
-  item.h = (int)(seg % (uint32_t)p.num_kv_heads);
-  item.row0 = 0;
-  item.row_end = 1 << p.group_log2;
-  item.slot = p.shared_splits + (int)split;
-  take_own<INDEXED>(p, (int)split, item.b0, item.h, &item.first);
-  attend<DT, FMT, 1, INDEXED, kWaves>(p, item, sh, sh_ids);
+  attend_own<DT, FMT, INDEXED>(p, blockIdx.x - shared_items, sh, sh_ids);
+}
+
+// More query rows than a wave can hold: a workgroup takes 128 query rows of a head (32 a wave) and a macro tile of 128 tokens at a
+// time.  Each wave loads 32 of the tokens, converts and transposes them into matrix operands once and leaves those in LDS,
+// from where all four waves read them; the rows of the next macro tile are on their way meanwhile.  Two workgroups share a
+// CU, so that one multiplies while the other waits or exponentiates.
+constexpr int kWideRows = 128, kMacro = kWaves * kTile;
+template <int DT, int FMT>
+__global__ __launch_bounds__(kThreads, 2) void kv_attend_wide_kernel(KvAttendParams p) {
+  struct Operands {
+    u32x4 frag[kWaves][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
+    float ks[kWaves][kTile], vs[kWaves][kTile];
+  };
+  __shared__ union {
+    Operands of;
+    AttendLds join;
+  } sh;
+  const uint32_t shared_items = (uint32_t)(p.row_blocks * p.num_kv_heads * p.shared_splits);
+  if (blockIdx.x >= shared_items) {
+    attend_own<DT, FMT, false>(p, blockIdx.x - shared_items, sh.join, nullptr);
+    return;
+  }
+  using State = Rows<DT, FMT, 2>;
+  const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t split = blockIdx.x % (uint32_t)p.shared_splits, rest_id = blockIdx.x / (uint32_t)p.shared_splits;
+  const int h = (int)(rest_id % (uint32_t)p.num_kv_heads);
+  const int row0 = (int)(rest_id / (uint32_t)p.num_kv_heads) * kWideRows + 32 * wave, row_end = p.batch << p.group_log2;
+  AttendSource it;
+  take_shared(p, (int)split, h, &it);
+  State rows;
+  rows.begin(p, 0, h, row0, row_end);
+  const bool idle = row0 >= row_end;   // (it still loads its share)
+
+  KTile<FMT> kt[2];
+  VRow<FMT> vr[8];
+  float scale = 0.0f;   // of a key row (lanes 0 .. 31) or a value row
+  DenseTiles<FMT> dense;
+  dense.begin(it);
+  const float* scales = lane < kTile ? it.ks : it.vs;
+  const auto load = [&](int tile) {
+    if (tile < it.end) {
+      const int start = tile_start(tile, it.end);
+      dense.key_rows(it, start, kt);
+      dense.value_rows(it, start, vr);
+      if constexpr (kQuantised<FMT>) scale = scales[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
+    }
+  };
+  load(it.begin + wave * kTile);
+  for (int macro = it.begin, rest = it.end - it.begin; rest > 0; macro += kMacro, rest -= kMacro) {
+    const int mine = macro + wave * kTile;
+    __syncthreads();   // (the operands of the last macro tile are done with)
+    if (wave * kTile < rest) {
+      if (rest - wave * kTile < kTile) clear_masked<FMT>(tile_mask(tile_start(mine, it.end), mine, it.end), vr);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) sh.of.frag[wave][4 * x + kb][lane] = k_frag<FMT, State::kQF16>(kt[x], kb);
+      const auto values = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        u32x4 even, odd;
+        v_frags<FMT, D>(vr, &even, &odd);
+        sh.of.frag[wave][8 + 2 * D][lane] = even;
+        sh.of.frag[wave][9 + 2 * D][lane] = odd;
+      };
+      values(std::integral_constant<int, 0>());
+      values(std::integral_constant<int, 1>());
+      values(std::integral_constant<int, 2>());
+      values(std::integral_constant<int, 3>());
+      if constexpr (kQuantised<FMT>) {
+        (lane < kTile ? sh.of.ks : sh.of.vs)[wave][lane & (kTile - 1)] = lane < kTile ? scale * p.scale_log2e : scale;
+      }
+    }
+    __syncthreads();
+    if (rest > kMacro) load(mine + kMacro);
+    if (idle) continue;
+    // the logits of the next tile go through the matrix cores beside the exponentials of this one
+    const int tiles = min((rest + kTile - 1) / kTile, kWaves);
+    f32x4 sc[2][2];
+    rows.scores(sc, [&](int x, int kb) { return sh.of.frag[0][4 * x + kb][lane]; });
+    for (int t = 0; t < tiles; ++t) {
+      const int after = t + 1 < tiles ? t + 1 : t;   // (behind the last one its own again, not used)
+      f32x4 next[2][2];
+      float kf[8], vf[8];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        f32x4 a = (f32x4){p.scale_log2e, p.scale_log2e, p.scale_log2e, p.scale_log2e}, b = a;
+        if constexpr (kQuantised<FMT>) {
+          a = *(const f32x4*)&sh.of.ks[t][16 * x + 4 * j];
+          b = *(const f32x4*)&sh.of.vs[t][16 * x + 4 * j];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          kf[4 * x + i] = a[i];
+          vf[4 * x + i] = b[i];
+        }
+      }
+      const int tile = macro + t * kTile;
+      const bool any_masked = rest - t * kTile < kTile;
+      uint32_t masked = 0;
+      if (any_masked) masked = tile_mask(tile_start(tile, it.end), tile, it.end);
+      rows.attend(
+          sc, kf, vf, masked, any_masked,
+          [&](auto d, u32x4* even, u32x4* odd) {
+            constexpr int D = decltype(d)::value;
+            *even = sh.of.frag[t][8 + 2 * D][lane];
+            *odd = sh.of.frag[t][9 + 2 * D][lane];
+          },
+          [&] { rows.scores(next, [&](int x, int kb) { return sh.of.frag[after][4 * x + kb][lane]; }); });
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        sc[r][0] = next[r][0];
+        sc[r][1] = next[r][1];
+      }
+    }
+  }
+  // each wave has its rows to itself: lane (n, j) dims 32 j .. 32 j + 31 of row n
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const float l = sum_over_quarters(rows.l_run[r]);
+    const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (kQuantised<FMT> ? rows.cap : 1.0f);
+    const int row = row0 + 16 * r + n;
+    if (row < row_end) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store_result<State::kPF16>(p, row >> p.group_log2, (h << p.group_log2) + (row & ((1 << p.group_log2) - 1)), (int)split, 32 * j + 8 * i,
+                                   (f32x4){rows.acc[r][0][i], rows.acc[r][1][i], rows.acc[r][2][i], rows.acc[r][3][i]} * norm,
+                                   (f32x4){rows.acc[r][4][i], rows.acc[r][5][i], rows.acc[r][6][i], rows.acc[r][7][i]} * norm, rows.m_ref[r], l);
+    }
+  }
 }
 
 // Short calls: one workgroup of eight waves per (entry, head) attends to everything and writes the result, one launch.  The
@@ -736,6 +935,8 @@ int launch_typed(const KvAttendParams& p, int row_tiles, hipStream_t stream) {
     kv_attend_kernel<DT, FMT, 1, false><<<grid, kThreads, 0, stream>>>(p);
   } else if (row_tiles == 2) {
     kv_attend_kernel<DT, FMT, 2, false><<<grid, kThreads, 0, stream>>>(p);
+  } else if (row_tiles == 8) {
+    kv_attend_wide_kernel<DT, FMT><<<grid, kThreads, 0, stream>>>(p);
   } else {
     kv_attend_kernel<DT, FMT, 4, false><<<grid, kThreads, 0, stream>>>(p);
   }
