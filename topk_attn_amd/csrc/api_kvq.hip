@@ -193,9 +193,9 @@ Plan plan_prefix(const tka_prefix_decode_args* a) {
     return p;
   }
   if (a->prefix.rows) {
-    p.row_tiles = query_rows <= 16 ? 1 : (query_rows <= 32 ? 2 : query_rows <= 64 ? 4 : 8);
+    p.row_tiles = query_rows <= 16 ? 1 : (query_rows <= 32 ? 2 : query_rows <= 64 ? 4 : (query_rows <= 128 ? 8 : 16));
     p.row_blocks = (int)((query_rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-    cut(a->prefix.rows, a->num_splits ? a->num_splits : (p.row_tiles == 4 ? 256 : 512) / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
+    cut(a->prefix.rows, a->num_splits ? a->num_splits : (p.row_tiles == 4 || p.row_tiles == 16 ? 256 : 512) / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
   }
   if (a->suffix.rows) cut(a->suffix.rows, 256 / (heads * batch), TKA_MAX_SPLITS / 2, &p.own_splits, &p.own_tps);
   return p;

@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t widen_pair(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, biased) - off);
   } else {
     const float lo = (float)(int8_t)(w >> (16 * HI)), hi = (float)(int8_t)(w >> (16 * HI + 8));
-    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);   // whole numbers below 2^8: the upper halves hold them
+    return pack_bf16(lo, hi);   // (whole numbers below 2^8: exact)
   }
 }
 // What widen_pair expects of a dword of codes.
@@ -115,6 +115,18 @@ __device__ __forceinline__ u32x4 k_frag(const KTile<FMT>& t, int kb) {
 // V registers: dims 8n .. 8n+7 of the eight slot tokens.
 template <int FMT>
 using VRow = typename std::conditional<kQuantised<FMT>, u32x2, u32x4>::type;
+
+// Rows that a loop carries along are to stay in the registers as they were loaded: the compiler otherwise carries the bytes that
+// their conversion begins with, in a register each (int8 keys, bf16 queries: 64 registers more than there are).
+template <int FMT>
+__device__ __forceinline__ void hold(KTile<FMT> (&kt)[2], VRow<FMT> (&vr)[8]) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < KTile<FMT>::kLoads; ++y) asm("" : "+v"(kt[x].w[y]));
+#pragma unroll
+  for (int s = 0; s < 8; ++s) asm("" : "+v"(vr[s]));
+}
 
 // V^T operands of output dims c = 2 D and 2 D + 1 (of the lane's eight): element s = token of slot s.
 template <int FMT, int D>
@@ -193,6 +205,12 @@ __device__ __forceinline__ void store_row(const KvAttendParams& p, int b, int hq
     p.out_lse[(((int64_t)b * p.num_kv_heads) << p.group_log2) + hq] = L > 0.0f || L != L ? (M + (__builtin_log2f(L) - l_log2)) * 0.69314718055994531f : -INFINITY;
 }
 
+// Twice the power of two at or above x (x >= 0), 2^-110 at least.
+__device__ __forceinline__ float power_above(float x) {
+  const uint32_t e = ((__builtin_bit_cast(uint32_t, x) + 0x7fffffu) & 0x7f800000u) + 0x800000u;
+  return __builtin_bit_cast(float, min(max(e, 17u << 23), 0x7e000000u));
+}
+
 // What a wave holds of its 16 RT query rows (row n of each sixteen in the lanes n, n + 16, n + 32, n + 48).
 template <int DT, int FMT, int RT>
 struct Rows {
@@ -227,6 +245,16 @@ struct Rows {
     cap = __builtin_bit_cast(float, 17u << 23);   // 2^-110: the least cap (its reciprocal stays in range)
   }
 
+  // The cap moves to `to`, a power of two, and the accumulators with it.
+  __device__ __forceinline__ void raise_cap(float to) {
+    const float drop = cap / to;
+    cap = to;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[r][c] *= drop;
+  }
+
   // Logits of a tile of 32 tokens, before their factors.  key_frag(x, kb): operand of sixteen x and k-block kb.
   template <typename KeyFrag>
   __device__ __forceinline__ void scores(f32x4 (&sc)[RT][2], KeyFrag key_frag) const {
@@ -244,10 +272,11 @@ struct Rows {
 
   // The rest of it.  kf: factors of the slot tokens' logits, vs: their value scales; masked: bit s = slot s has no row
   // (any_masked: some lane has one); value_frags(D, even, odd): operands of output dims 2 D and 2 D + 1.
-  // beside(): work that has nothing to do with this tile, beside its exponentials.
-  template <typename ValueFrags, typename Beside>
-  __device__ __forceinline__ void attend(f32x4 (&sc)[RT][2], float (&kf)[8], float (&vs)[8], uint32_t masked, bool any_masked, ValueFrags value_frags,
-                                         Beside beside) {
+  // tile_scale (SCALED): a power of two that the value operands have been divided by, with their scales in them (vs is then not
+  // looked at).
+  template <bool SCALED, typename ValueFrags>
+  __device__ __forceinline__ void attend(f32x4 (&sc)[RT][2], float (&kf)[8], float (&vs)[8], float tile_scale, uint32_t masked, bool any_masked,
+                                         ValueFrags value_frags) {
     // masked slots have no weight (and their value rows are zeros: no 0 * inf, no 0 * NaN)
     if (any_masked) {
 #pragma unroll
@@ -260,21 +289,17 @@ struct Rows {
         }
     }
     float weight[8];   // scale of a slot's value row over the cap
-    if constexpr (kQuantised<FMT>) {
+    float unit_log2 = kWeightLog2<kPF16>, back = 1.0f;   // log2 of the unit that the weights are held in; what takes their sum back to 2^kWeightLog2
+    if constexpr (SCALED) {
+      if (tile_scale > cap) raise_cap(tile_scale);
+      const int below = max((int)(__builtin_bit_cast(uint32_t, tile_scale) >> 23) - (int)(__builtin_bit_cast(uint32_t, cap) >> 23), -40);   // (2^-40 of the cap: nothing)
+      unit_log2 += (float)below;
+      back = __builtin_bit_cast(float, (uint32_t)(127 - below) << 23);
+    } else if constexpr (kQuantised<FMT>) {
       float top = fabsf(vs[0]);
 #pragma unroll
       for (int s = 1; s < 8; ++s) top = fmaxf(top, fabsf(vs[s]));
-      if (__ballot(top > cap) != 0ull) {
-        top = max_over_quarters(top);
-        const uint32_t e = ((__builtin_bit_cast(uint32_t, top) + 0x7fffffu) & 0x7f800000u) + 0x800000u;   // twice the power of two at or above it
-        const float raised = __builtin_bit_cast(float, e < 0x7e000000u ? e : 0x7e000000u);
-        const float drop = cap / raised;
-        cap = raised;
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) acc[r][c] *= drop;
-      }
+      if (__ballot(top > cap) != 0ull) raise_cap(power_above(max_over_quarters(top)));
       const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, cap));   // 1 / cap
 #pragma unroll
       for (int s = 0; s < 8; ++s) weight[s] = vs[s] * unit;
@@ -284,11 +309,10 @@ struct Rows {
     // pass that moves the references.
     u32x4 pf[RT], pf_lo[RT];
     float ps[RT][8], sum[RT], most = 0.0f;
-    beside();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][s >> 2][s & 3], kf[s], kWeightLog2<kPF16> - m_ref[r]));
+      for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][s >> 2][s & 3], kf[s], unit_log2 - m_ref[r]));
       sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
       most = fmaxf(most, sum[r]);
     }
@@ -308,18 +332,18 @@ struct Rows {
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[r][c] *= alpha;
 #pragma unroll
-        for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(xs[s] + (kWeightLog2<kPF16> - m_new));
+        for (int s = 0; s < 8; ++s) ps[r][s] = __builtin_amdgcn_exp2f(xs[s] + (unit_log2 - m_new));
         sum[r] = ((ps[r][0] + ps[r][1]) + (ps[r][2] + ps[r][3])) + ((ps[r][4] + ps[r][5]) + (ps[r][6] + ps[r][7]));
       }
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      l_run[r] += sum[r];
+      l_run[r] = SCALED ? __builtin_fmaf(sum[r], back, l_run[r]) : l_run[r] + sum[r];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float a = ps[r][2 * w], b = ps[r][2 * w + 1];
         if constexpr (kPF16) {
-          const float x = kQuantised<FMT> ? a * weight[2 * w] : a, y = kQuantised<FMT> ? b * weight[2 * w + 1] : b;
+          const float x = kQuantised<FMT> && !SCALED ? a * weight[2 * w] : a, y = kQuantised<FMT> && !SCALED ? b * weight[2 * w + 1] : b;
           pf[r][w] = pack_f16(x, y);
           if constexpr (kSplit) {
             uint32_t hi = pf[r][w];
@@ -532,7 +556,7 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
         rows.scores(sc, [&](int x, int kb) { return k_frag<FMT, Rows<DT, FMT, RT>::kQF16>(kt[x], kb); });
         if (more) load_keys(next);
         if (any_masked) clear_masked<FMT>(masked, vr);
-        rows.attend(sc, kf, vs, masked, any_masked, [&](auto d, u32x4* even, u32x4* odd) { v_frags<FMT, decltype(d)::value>(vr, even, odd); }, [] {});
+        rows.template attend<false>(sc, kf, vs, 0.0f, masked, any_masked, [&](auto d, u32x4* even, u32x4* odd) { v_frags<FMT, decltype(d)::value>(vr, even, odd); });
         if (!more) break;
         load_values(next);
         tile = next_tile;
@@ -671,7 +695,7 @@ __device__ __forceinline__ void take_own(const KvAttendParams& p, int split, int
 }
 
 // The own items of a launch: splits of (entry, head) pairs.
-template <int DT, int FMT, bool INDEXED>
+template <int DT, int FMT, bool INDEXED, int WAVES>
 __device__ __forceinline__ void attend_own(const KvAttendParams& p, uint32_t own, AttendLds& sh, int32_t* sh_ids) {
   const uint32_t split = own % (uint32_t)p.own_splits, seg = own / (uint32_t)p.own_splits;
   AttendItem item;
@@ -682,7 +706,7 @@ __device__ __forceinline__ void attend_own(const KvAttendParams& p, uint32_t own
   item.row_end = 1 << p.group_log2;
   item.slot = p.shared_splits + (int)split;
   take_own<INDEXED>(p, (int)split, item.b0, item.h, &item.first);
-  attend<DT, FMT, 1, INDEXED, kWaves>(p, item, sh, sh_ids);
+  attend<DT, FMT, 1, INDEXED, WAVES>(p, item, sh, sh_ids);
 }
 
 // RT: sixteens of query rows that a workgroup of the shared source takes (0: there is no shared source)
@@ -704,19 +728,25 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
     attend<DT, FMT, RT ? RT : 1, false, kWaves>(p, item, sh, sh_ids);
     return;
   }
-  attend_own<DT, FMT, INDEXED>(p, blockIdx.x - shared_items, sh, sh_ids);
+  attend_own<DT, FMT, INDEXED, kWaves>(p, blockIdx.x - shared_items, sh, sh_ids);
 }
 
-// More query rows than a wave can hold: a workgroup takes 128 query rows of a head (32 a wave) and a macro tile of 128 tokens at a
-// time.  Each wave loads 32 of the tokens, converts and transposes them into matrix operands once and leaves those in LDS,
-// from where all four waves read them; the rows of the next macro tile are on their way meanwhile.  Two workgroups share a
-// CU, so that one multiplies while the other waits or exponentiates.
-constexpr int kWideRows = 128, kMacro = kWaves * kTile;
-template <int DT, int FMT>
-__global__ __launch_bounds__(kThreads, 2) void kv_attend_wide_kernel(KvAttendParams p) {
+// More query rows than a wave can hold: the waves of a workgroup take 32 query rows of a head each and go through the tokens
+// together, a macro tile of 32 tokens a wave at a time.  Each wave loads its 32 tokens, converts and transposes them into
+// matrix operands once and leaves those in LDS, from where all waves read them; the rows of the next macro tile are on
+// their way meanwhile.
+template <int DT, int FMT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAttendParams p) {
+  using State = Rows<DT, FMT, 2>;
+  constexpr int kMacro = WAVES * kTile;
+  // Value operands with their scales in them, over a power of two of the tile: exact in e4m3, where scales are powers of two
+  // (but for what lies 2^-24 below the tile's largest), and off by half a step of fp16 twice in int8, which is left to the
+  // weights where these are kept in two parts.  It saves a product for every weight.
+  constexpr bool kScaled = kQuantised<FMT> && (FMT == TKA_KV_E4M3 || !State::kSplit);
   struct Operands {
-    u32x4 frag[kWaves][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
-    float ks[kWaves][kTile], vs[kWaves][kTile];
+    u32x4 frag[WAVES][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
+    float ks[WAVES][kTile], vs[WAVES][kTile];
+    float tile_scale[WAVES];
   };
   __shared__ union {
     Operands of;
@@ -724,15 +754,14 @@ __global__ __launch_bounds__(kThreads, 2) void kv_attend_wide_kernel(KvAttendPar
   } sh;
   const uint32_t shared_items = (uint32_t)(p.row_blocks * p.num_kv_heads * p.shared_splits);
   if (blockIdx.x >= shared_items) {
-    attend_own<DT, FMT, false>(p, blockIdx.x - shared_items, sh.join, nullptr);
+    attend_own<DT, FMT, false, WAVES>(p, blockIdx.x - shared_items, sh.join, nullptr);
     return;
   }
-  using State = Rows<DT, FMT, 2>;
   const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t split = blockIdx.x % (uint32_t)p.shared_splits, rest_id = blockIdx.x / (uint32_t)p.shared_splits;
   const int h = (int)(rest_id % (uint32_t)p.num_kv_heads);
-  const int row0 = (int)(rest_id / (uint32_t)p.num_kv_heads) * kWideRows + 32 * wave, row_end = p.batch << p.group_log2;
+  const int row0 = (int)(rest_id / (uint32_t)p.num_kv_heads) * (32 * WAVES) + 32 * wave, row_end = p.batch << p.group_log2;
   AttendSource it;
   take_shared(p, (int)split, h, &it);
   State rows;
@@ -742,83 +771,103 @@ __global__ __launch_bounds__(kThreads, 2) void kv_attend_wide_kernel(KvAttendPar
   KTile<FMT> kt[2];
   VRow<FMT> vr[8];
   float scale = 0.0f;   // of a key row (lanes 0 .. 31) or a value row
-  DenseTiles<FMT> dense;
-  dense.begin(it);
-  const float* scales = lane < kTile ? it.ks : it.vs;
   const auto load = [&](int tile) {
     if (tile < it.end) {
       const int start = tile_start(tile, it.end);
+      DenseTiles<FMT> dense;
+      AttendSource from = it;
+      asm("" : "+s"(from.stride_n), "+s"(from.end));   // (the offsets are made here, not kept in registers over the loop)
+      dense.begin(from);
       dense.key_rows(it, start, kt);
       dense.value_rows(it, start, vr);
-      if constexpr (kQuantised<FMT>) scale = scales[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
+      if constexpr (kQuantised<FMT>) scale = (lane < kTile ? it.ks : it.vs)[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
     }
   };
+  // the operands of the tile in the registers, from position `tile` on
+  const auto stage = [&](int tile) {
+    const int token = lane & (kTile - 1);
+    const bool cut = it.end - tile < kTile;
+    const int start = tile_start(tile, it.end);
+    if constexpr (kQuantised<FMT>) hold<FMT>(kt, vr);
+    if (cut) clear_masked<FMT>(tile_mask(start, tile, it.end), vr);
+    u32x4 factor;   // of the value rows: pairs of slots
+    if constexpr (kScaled) {
+      float top = lane < kTile ? 0.0f : fabsf(scale);
+#pragma unroll
+      for (int x = 1; x < kTile; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
+      top = power_above(__shfl(top, kWave - 1, kWave));
+      _Float16 f = (_Float16)(scale * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, top)));
+      if (cut && (start + token < tile || start + token >= it.end)) f = (_Float16)0.0f;
+      _Float16* held = (_Float16*)sh.of.vs[wave];
+      if (lane >= kTile) held[token] = f;
+      if (lane == 0) sh.of.tile_scale[wave] = top;
+      const u32x2 lo = *(const u32x2*)(held + 4 * j), hi = *(const u32x2*)(held + 16 + 4 * j);
+      factor = (u32x4){lo[0], lo[1], hi[0], hi[1]};
+      if (lane < kTile) sh.of.ks[wave][token] = scale * p.scale_log2e;
+    } else if constexpr (kQuantised<FMT>) {
+      (lane < kTile ? sh.of.ks : sh.of.vs)[wave][token] = lane < kTile ? scale * p.scale_log2e : scale;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        sh.of.frag[wave][4 * x + kb][lane] = k_frag<FMT, State::kQF16>(kt[x], kb);
+        __builtin_amdgcn_sched_barrier(0);   // (one operand after the other: all at once they do not fit the registers)
+      }
+    const auto values = [&](auto d) {
+      constexpr int D = decltype(d)::value;
+      u32x4 even, odd;
+      v_frags<FMT, D>(vr, &even, &odd);
+      if constexpr (kScaled) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          even[w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, even[w]) * __builtin_bit_cast(f16x2, factor[w]));
+          odd[w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, odd[w]) * __builtin_bit_cast(f16x2, factor[w]));
+        }
+      }
+      sh.of.frag[wave][8 + 2 * D][lane] = even;
+      sh.of.frag[wave][9 + 2 * D][lane] = odd;
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    values(std::integral_constant<int, 0>());
+    values(std::integral_constant<int, 1>());
+    values(std::integral_constant<int, 2>());
+    values(std::integral_constant<int, 3>());
+  };
+
   load(it.begin + wave * kTile);
   for (int macro = it.begin, rest = it.end - it.begin; rest > 0; macro += kMacro, rest -= kMacro) {
     const int mine = macro + wave * kTile;
     __syncthreads();   // (the operands of the last macro tile are done with)
-    if (wave * kTile < rest) {
-      if (rest - wave * kTile < kTile) clear_masked<FMT>(tile_mask(tile_start(mine, it.end), mine, it.end), vr);
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) sh.of.frag[wave][4 * x + kb][lane] = k_frag<FMT, State::kQF16>(kt[x], kb);
-      const auto values = [&](auto d) {
-        constexpr int D = decltype(d)::value;
-        u32x4 even, odd;
-        v_frags<FMT, D>(vr, &even, &odd);
-        sh.of.frag[wave][8 + 2 * D][lane] = even;
-        sh.of.frag[wave][9 + 2 * D][lane] = odd;
-      };
-      values(std::integral_constant<int, 0>());
-      values(std::integral_constant<int, 1>());
-      values(std::integral_constant<int, 2>());
-      values(std::integral_constant<int, 3>());
-      if constexpr (kQuantised<FMT>) {
-        (lane < kTile ? sh.of.ks : sh.of.vs)[wave][lane & (kTile - 1)] = lane < kTile ? scale * p.scale_log2e : scale;
-      }
-    }
+    if (wave * kTile < rest) stage(mine);
     __syncthreads();
     if (rest > kMacro) load(mine + kMacro);
     if (idle) continue;
-    // the logits of the next tile go through the matrix cores beside the exponentials of this one
-    const int tiles = min((rest + kTile - 1) / kTile, kWaves);
-    f32x4 sc[2][2];
-    rows.scores(sc, [&](int x, int kb) { return sh.of.frag[0][4 * x + kb][lane]; });
+    const int tiles = min((rest + kTile - 1) / kTile, WAVES);
     for (int t = 0; t < tiles; ++t) {
-      const int after = t + 1 < tiles ? t + 1 : t;   // (behind the last one its own again, not used)
-      f32x4 next[2][2];
-      float kf[8], vf[8];
+      const int tile = macro + t * kTile;
+      const bool cut = rest - t * kTile < kTile;
+      f32x4 sc[2][2];
+      rows.scores(sc, [&](int x, int kb) { return sh.of.frag[t][4 * x + kb][lane]; });
+      float kf[8], vf[8], tile_scale = 0.0f;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         f32x4 a = (f32x4){p.scale_log2e, p.scale_log2e, p.scale_log2e, p.scale_log2e}, b = a;
-        if constexpr (kQuantised<FMT>) {
-          a = *(const f32x4*)&sh.of.ks[t][16 * x + 4 * j];
-          b = *(const f32x4*)&sh.of.vs[t][16 * x + 4 * j];
-        }
+        if constexpr (kQuantised<FMT>) a = *(const f32x4*)&sh.of.ks[t][16 * x + 4 * j];
+        if constexpr (kQuantised<FMT> && !kScaled) b = *(const f32x4*)&sh.of.vs[t][16 * x + 4 * j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           kf[4 * x + i] = a[i];
           vf[4 * x + i] = b[i];
         }
       }
-      const int tile = macro + t * kTile;
-      const bool any_masked = rest - t * kTile < kTile;
-      uint32_t masked = 0;
-      if (any_masked) masked = tile_mask(tile_start(tile, it.end), tile, it.end);
-      rows.attend(
-          sc, kf, vf, masked, any_masked,
-          [&](auto d, u32x4* even, u32x4* odd) {
-            constexpr int D = decltype(d)::value;
-            *even = sh.of.frag[t][8 + 2 * D][lane];
-            *odd = sh.of.frag[t][9 + 2 * D][lane];
-          },
-          [&] { rows.scores(next, [&](int x, int kb) { return sh.of.frag[after][4 * x + kb][lane]; }); });
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        sc[r][0] = next[r][0];
-        sc[r][1] = next[r][1];
-      }
+      if constexpr (kScaled) tile_scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.of.tile_scale[t])));
+      rows.template attend<kScaled>(sc, kf, vf, tile_scale, cut ? tile_mask(tile_start(tile, it.end), tile, it.end) : 0u, cut,
+                                    [&](auto d, u32x4* even, u32x4* odd) {
+                                      constexpr int D = decltype(d)::value;
+                                      *even = sh.of.frag[t][8 + 2 * D][lane];
+                                      *odd = sh.of.frag[t][9 + 2 * D][lane];
+                                    });
     }
   }
   // each wave has its rows to itself: lane (n, j) dims 32 j .. 32 j + 31 of row n
@@ -936,7 +985,9 @@ int launch_typed(const KvAttendParams& p, int row_tiles, hipStream_t stream) {
   } else if (row_tiles == 2) {
     kv_attend_kernel<DT, FMT, 2, false><<<grid, kThreads, 0, stream>>>(p);
   } else if (row_tiles == 8) {
-    kv_attend_wide_kernel<DT, FMT><<<grid, kThreads, 0, stream>>>(p);
+    kv_attend_wide_kernel<DT, FMT, 4><<<grid, 4 * kWave, 0, stream>>>(p);
+  } else if (row_tiles == 16) {
+    kv_attend_wide_kernel<DT, FMT, 8><<<grid, 8 * kWave, 0, stream>>>(p);
   } else {
     kv_attend_kernel<DT, FMT, 4, false><<<grid, kThreads, 0, stream>>>(p);
   }
