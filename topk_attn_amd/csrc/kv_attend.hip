@@ -421,7 +421,7 @@ struct DenseTiles {
     if constexpr (kQuantised<FMT>) scales(it, it.ks, start, ks);
   }
   __device__ __forceinline__ void values(const AttendSource& it, int start, VRow<FMT> (&vr)[8], float (&vs)[8]) const {
-    value_rows(it, start, vr);
+    value_rows<true>(it, start, vr);
     if constexpr (kQuantised<FMT>) scales(it, it.vs, start, vs);
   }
   __device__ __forceinline__ void key_rows(const AttendSource& it, int start, KTile<FMT> (&kt)[2]) const {
@@ -431,10 +431,15 @@ struct DenseTiles {
 #pragma unroll
       for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(base + k_off[x] + 64 * y);
   }
+  // STREAM: rows that nobody else reads (a request covers whole lines; 4 x 8 x 32768 rows of 8 bits: 52.2 -> 47.7 us).
+  template <bool STREAM>
   __device__ __forceinline__ void value_rows(const AttendSource& it, int start, VRow<FMT> (&vr)[8]) const {
     const unsigned char* base = it.v + (int64_t)start * it.stride_n;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) vr[s] = *(const VRow<FMT>*)(base + v_off[s]);
+    for (int s = 0; s < 8; ++s) {
+      const VRow<FMT>* row = (const VRow<FMT>*)(base + v_off[s]);
+      vr[s] = STREAM ? __builtin_nontemporal_load(row) : *row;
+    }
   }
 };
 
@@ -779,7 +784,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       asm("" : "+s"(from.stride_n), "+s"(from.end));   // (the offsets are made here, not kept in registers over the loop)
       dense.begin(from);
       dense.key_rows(it, start, kt);
-      dense.value_rows(it, start, vr);
+      dense.template value_rows<false>(it, start, vr);
       if constexpr (kQuantised<FMT>) scale = (lane < kTile ? it.ks : it.vs)[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
     }
   };

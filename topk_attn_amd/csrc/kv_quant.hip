@@ -132,12 +132,12 @@ __global__ __launch_bounds__(kThreads) void kvq_write_kernel(KvqCopyParams p, ui
   const int64_t in = it.b * p.stride_b + it.token * p.stride_n + it.h * p.stride_h + 32 * lane;
   const int64_t to = it.b * p.cache.stride_b + it.target * p.cache.stride_n + it.h * p.cache.stride_h + 16 * lane;
   const int64_t st = it.b * p.cache.scale_b + it.target * p.cache.scale_n + it.h * p.cache.scale_h;
-  const u32x4 ka = *(const u32x4*)(p.k + in), kb = *(const u32x4*)(p.k + in + 16);
-  const u32x4 va = *(const u32x4*)(p.v + in), vb = *(const u32x4*)(p.v + in + 16);
+  const u32x4 ka = __builtin_nontemporal_load((const u32x4*)(p.k + in)), kb = __builtin_nontemporal_load((const u32x4*)(p.k + in + 16));
+  const u32x4 va = __builtin_nontemporal_load((const u32x4*)(p.v + in)), vb = __builtin_nontemporal_load((const u32x4*)(p.v + in + 16));
   float scale;
-  *(u32x4*)((unsigned char*)p.cache.k + to) = quantise16<DT, FMT>(ka, kb, &scale);
+  __builtin_nontemporal_store((quantise16<DT, FMT>(ka, kb, &scale)), (u32x4*)((unsigned char*)p.cache.k + to));
   if (lane == 0) ((float*)p.cache.ks)[st] = scale;
-  *(u32x4*)((unsigned char*)p.cache.v + to) = quantise16<DT, FMT>(va, vb, &scale);
+  __builtin_nontemporal_store((quantise16<DT, FMT>(va, vb, &scale)), (u32x4*)((unsigned char*)p.cache.v + to));
   if (lane == 0) ((float*)p.cache.vs)[st] = scale;
 }
 
@@ -150,16 +150,17 @@ __device__ __forceinline__ uint16_t narrow_finite(float x) {
 }
 
 template <int DT, int FMT>
-__device__ __forceinline__ void dequantise16(const u32x4& w, float scale, u32x4* a, u32x4* b) {
+__device__ __forceinline__ u32x4 dequantise8(const u32x2& w, float scale) {
+  u32x4 o;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     float f[4];
     Codes<FMT>::widen(w[i], f);
-    u32x4& o = i < 2 ? *a : *b;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      o[2 * (i & 1) + e] = (uint32_t)narrow_finite<DT>(f[2 * e] * scale) | ((uint32_t)narrow_finite<DT>(f[2 * e + 1] * scale) << 16);
+      o[2 * i + e] = (uint32_t)narrow_finite<DT>(f[2 * e] * scale) | ((uint32_t)narrow_finite<DT>(f[2 * e + 1] * scale) << 16);
   }
+  return o;
 }
 
 template <int DT, int FMT>
@@ -167,18 +168,18 @@ __global__ __launch_bounds__(kThreads) void kvq_read_kernel(KvqCopyParams p, uin
   const CopyItem it = copy_item(p, token_tiles);
   if (!it.there) return;
   const int lane = threadIdx.x % kRowLanes;
-  const int64_t to = it.b * p.stride_b + it.token * p.stride_n + it.h * p.stride_h + 32 * lane;
-  const int64_t at = it.b * p.cache.stride_b + it.target * p.cache.stride_n + it.h * p.cache.stride_h + 16 * lane;
+  // a lane takes eight codes of either half of the row: a store then covers half a row without gaps, which is what the
+  // streaming hint needs (with sixteen neighbouring codes a lane: 112 us instead of 84)
+  const int64_t to = it.b * p.stride_b + it.token * p.stride_n + it.h * p.stride_h + 16 * lane;
+  const int64_t at = it.b * p.cache.stride_b + it.target * p.cache.stride_n + it.h * p.cache.stride_h + 8 * lane;
   const int64_t st = it.b * p.cache.scale_b + it.target * p.cache.scale_n + it.h * p.cache.scale_h;
-  const u32x4 kw = *(const u32x4*)(p.cache.k + at), vw = *(const u32x4*)(p.cache.v + at);
+  const u32x2 ka = *(const u32x2*)(p.cache.k + at), kb = *(const u32x2*)(p.cache.k + at + 64);
+  const u32x2 va = *(const u32x2*)(p.cache.v + at), vb = *(const u32x2*)(p.cache.v + at + 64);
   const float ks = p.cache.ks[st], vs = p.cache.vs[st];
-  u32x4 a, b;
-  dequantise16<DT, FMT>(kw, ks, &a, &b);
-  *(u32x4*)(p.k + to) = a;
-  *(u32x4*)(p.k + to + 16) = b;
-  dequantise16<DT, FMT>(vw, vs, &a, &b);
-  *(u32x4*)(p.v + to) = a;
-  *(u32x4*)(p.v + to + 16) = b;
+  __builtin_nontemporal_store((dequantise8<DT, FMT>(ka, ks)), (u32x4*)(p.k + to));
+  __builtin_nontemporal_store((dequantise8<DT, FMT>(kb, ks)), (u32x4*)(p.k + to + 128));
+  __builtin_nontemporal_store((dequantise8<DT, FMT>(va, vs)), (u32x4*)(p.v + to));
+  __builtin_nontemporal_store((dequantise8<DT, FMT>(vb, vs)), (u32x4*)(p.v + to + 128));
 }
 
 // A wave scores 64 tokens of a head: eight lanes a row, row u of group g is token 8g + u, so that lane 8g + x ends with the
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void kvq_read_kernel(KvqCopyParams p, uin
 // takes the pair i = x (x < 4) or 11 - x, so that distance 8 is the DPP half mirror (i(7 - x) = i(x) ^ 4) and 4 and 2 are quad
 // permutations: no exchange goes through the LDS crossbar, and the sums pair up as in the definition.
 constexpr int kScoreRound = 64;
-constexpr int kScoreTokens = (kThreads / kWave) * kScoreRound;   // tokens of a workgroup
+constexpr int kScoreTokens = (kThreads / kWave) * kScoreRound;   // tokens of a workgroup (512: 95 us where 256 take 92, 1024: 102)
 
 __device__ __forceinline__ float sum8(float p) {   // over eight lanes; every lane ends with the sum
   p = p + dpp_f32<0x141>(p);   // row_half_mirror
@@ -208,48 +209,47 @@ __global__ __launch_bounds__(kThreads) void kvq_scores_kernel(KvqScoresParams p,
     const int64_t n = p.kv_len[b];
     len = n < 0 ? 0 : (n < len ? n : len);
   }
-  const int64_t first = (int64_t)tile * kScoreTokens + wave * kScoreRound;
-  if (first >= p.cache.rows) return;
-  float* out = p.scores + (int64_t)seg * p.cache.rows + first + lane;
-  const bool in_range = first + lane < p.cache.rows;
-  if (first >= len) {
-    if (in_range) *out = -INFINITY;
-    return;
-  }
-  float qa[8], qb[8];
-  load_group_query<DT>(p.q, p.q_stride_b, b, h, p.group, 2 * i, qa);
-  load_group_query<DT>(p.q, p.q_stride_b, b, h, p.group, 2 * i + 1, qb);
+  // The rows are asked for before anything else; the sum of the group's queries (ascending, as in the definition) is made once
+  // for the workgroup while they are on their way.
+  const int64_t first = ((int64_t)tile * (kThreads / kWave) + wave) * kScoreRound, mine = first + lane;
+  const int64_t last = len > 0 ? len - 1 : 0;
   const unsigned char* k = p.cache.k + b * p.cache.stride_b + h * p.cache.stride_h + 16 * i;
+  const float* scales = p.cache.ks + b * p.cache.scale_b + h * p.cache.scale_h;
   u32x4 w[8];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    int64_t t = first + 8 * g + u;
-    t = t < len ? t : len - 1;
-    w[u] = __builtin_nontemporal_load((const u32x4*)(k + t * p.cache.stride_n));
+  for (int u = 0; u < 8; ++u) w[u] = __builtin_nontemporal_load((const u32x4*)(k + min(first + 8 * g + u, last) * p.cache.stride_n));
+  const float ks = scales[min(mine, last) * p.cache.scale_n];
+  __shared__ __align__(16) float sh_q[kHeadDim];
+  if (threadIdx.x < kHeadDim) {
+    const uint16_t* q = (const uint16_t*)p.q + (int64_t)b * p.q_stride_b + (int64_t)h * p.group * kHeadDim + threadIdx.x;
+    uint16_t part[TKA_MAX_GROUP];
+#pragma unroll
+    for (int x = 0; x < TKA_MAX_GROUP; ++x) part[x] = q[(x < p.group ? x : 0) * kHeadDim];
+    float sum = Elem<DT>::widen(part[0]);
+#pragma unroll
+    for (int x = 1; x < TKA_MAX_GROUP; ++x)
+      if (x < p.group) sum += Elem<DT>::widen(part[x]);
+    sh_q[threadIdx.x] = sum;
   }
-  int64_t mine = first + lane;
-  mine = mine < len ? mine : len - 1;
-  const float ks = p.cache.ks[b * p.cache.scale_b + mine * p.cache.scale_n + h * p.cache.scale_h];
+  __syncthreads();
+  float qf[16];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) *(f32x4*)&qf[4 * d] = *(const f32x4*)&sh_q[16 * i + 4 * d];
   float dot = 0.0f;
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
-    float a = 0.0f, c = 0.0f, f[4];
+    asm("" : "+v"(w[u]));   // (one row after the other: the compiler otherwise takes the bytes of all of them apart first)
+    float part[2] = {0.0f, 0.0f}, f[4];
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
+    for (int d = 0; d < 4; ++d) {
       Codes<FMT>::widen(w[u][d], f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) a = __builtin_fmaf(qa[4 * d + e], f[e], a);
+      for (int e = 0; e < 4; ++e) part[d >> 1] = __builtin_fmaf(qf[4 * d + e], f[e], part[d >> 1]);
     }
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      Codes<FMT>::widen(w[u][2 + d], f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c = __builtin_fmaf(qb[4 * d + e], f[e], c);
-    }
-    const float s = sum8(a) + sum8(c);
+    const float s = sum8(part[0]) + sum8(part[1]);
     dot = x == u ? s : dot;
   }
-  if (in_range) *out = first + lane < len ? (dot * ks) * p.scale : -INFINITY;
+  if (mine < p.cache.rows) p.scores[(int64_t)seg * p.cache.rows + mine] = mine < len ? (dot * ks) * p.scale : -INFINITY;
 }
 
 template <typename Launch>
