@@ -50,7 +50,7 @@ typedef struct tka_kv_cache {
   int32_t batch;
   int32_t num_kv_heads;
   int32_t head_dim;       /* must be 128                                                        */
-  int64_t rows;           /* tokens per entry there is room for, < 2^31                         */
+  int64_t rows;           /* tokens per entry there is room for, <= 2^31 - 1025                 */
   int64_t stride_b, stride_n, stride_h;
   int64_t scale_stride_b, scale_stride_n, scale_stride_h;
 } tka_kv_cache;

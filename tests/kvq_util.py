@@ -5,11 +5,11 @@ Bounds of the decode outputs.  With u = 2^-24 (half a step of fp32), per query r
              140 * 2u * S, S = max over tokens of scale * sum |q k| (2u: the matrix unit need not round to nearest);
              in the exponent of 2 a logit has rounding |x| * 2u and the exponential 2^-21 of its own: a weight is off by at
              most e_w = 140 * 2u * S + |x|max * 2u + 2^-21 of itself, S and x in the base that makes them larger (log2 e);
-  weights    fp16 weights: 2^-11 of themselves.  Below the normal range they are off by 2^-25, held times 2^9 over a cap of
-             at most four times the largest scale, whose row holds a code of at least half the largest one: 2^-34 * 4 * 2 of
-             max |v|, against a sum of weights of at least 2^-6 of the reference's: 2^-31 * 2^6 would be the very worst; a
-             reference that lags by 2^6 has a weight of 2^6 in the sum, so the quotient stays below 2^-31.  bf16 weights in
-             two parts: 2^-16;
+  weights    in two parts (bf16 rows of 16 bits; every case of fp16 queries): 2^-16 of themselves.  One fp16 number (8-bit rows,
+             bf16 queries): 2^-11, and twice that again where value rows carry their scales in fp16 (a factor and a
+             product): 3 * 2^-11.  Below the normal range a weight is off by 2^-25, held times 2^9 over a cap of at most four
+             times the largest scale, whose row holds a code of at least half the largest one: 2^-34 * 4 * 2 of max |v|,
+             against a sum of weights of at least that of the reference, which lags by 2^6 at most: below 2^-31 of max |v|;
   sums       fp32 sums of n terms: n * 2u;
   output     rounded to its type: eps / 2 of itself.
 So |error| <= eps_out / 2 * |o| + (2 e_w + w + 2 n * 2u) * sum p |v| + n * 2^-31 * max |v|, p the normalised weights; lse is off by
@@ -73,13 +73,13 @@ def attention64(q, k, v, scale=SCALE):
     return p @ v, torch.logsumexp(s, -1), p @ v.abs(), big, float(s.abs().max())
 
 
-def check_attention(out, lse, q, k, v, dtype16, fp16_weights, scale=SCALE):
+def check_attention(out, lse, q, k, v, dtype16, two_parts, scale=SCALE):
     """out [R,128] (16 bits), lse [R] of one head against 64 bits; k, v: the rows that count, in 64 bits."""
     o, l, pv, big, top = attention64(q.double(), k.double(), v.double(), scale)
     n = k.shape[0]
     log2e = 1.4426950408889634
     e_w = 140 * 2 * U * big * log2e + top * log2e * 2 * U + 2.0 ** -21
-    w = 2.0 ** -11 if fp16_weights else 2.0 ** -16
+    w = 2.0 ** -16 if two_parts else 3 * 2.0 ** -11
     vmax = float(v.abs().max()) if n else 0.0
     bound = torch.finfo(dtype16).eps / 2 * o.abs() + (2 * e_w + w + 4 * n * U) * pv + n * 2.0 ** -31 * vmax + torch.finfo(dtype16).smallest_normal * torch.finfo(dtype16).eps
     err = (out.double().cpu() - o).abs()

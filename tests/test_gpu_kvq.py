@@ -204,7 +204,7 @@ def _check_decode(out, lse, q, k, v, rows_of, G, dtype):
         for h in range(H):
             rows = rows_of(b, h)
             qs = slice(h * G, (h + 1) * G)
-            check_attention(out[b, qs], lse[b, qs] if lse is not None else None, q[b, qs], k[b, rows, h], v[b, rows, h], out.dtype, True)
+            check_attention(out[b, qs], lse[b, qs] if lse is not None else None, q[b, qs], k[b, rows, h], v[b, rows, h], out.dtype, dtype == "f16")
 
 
 @pytest.mark.parametrize("dtype,fmt", TYPES)
@@ -300,6 +300,20 @@ def test_decode_scales_far_apart(dtype, fmt):
     _check_decode(out, lse, q * 4, k, v, lambda b, h: slice(0, N), G, dtype)
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_decode_score_factors(scale):
+    """A negative factor turns the weights round, a factor of zero makes them equal; so does a negative scale of a row."""
+    q, cache, k, v = _decode_case(torch.Generator().manual_seed(5), 1, 2, 4, 300, "bf16", "int8", "heads")
+    cache.k_scale[:, ::3] *= -1
+    cache.v_scale[:, ::5] *= -100
+    k[:, ::3] *= -1
+    v[:, ::5] *= -100
+    announce("kvq decode factor %g" % scale)
+    out, lse = ops.kvq_flash_decode(q.cuda(), cache, scale, 4, return_lse=True)
+    for h in range(2):
+        check_attention(out[0, 4 * h:4 * h + 4], lse[0, 4 * h:4 * h + 4], q[0, 4 * h:4 * h + 4], k[0, :, h], v[0, :, h], out.dtype, False, scale)
+
+
 @pytest.mark.parametrize("fmt", list(CODES))
 def test_decode_shared_cache(fmt):
     """One cache [N,H,128] for the batch equals a copy for each entry, bit for bit."""
@@ -376,7 +390,7 @@ def test_sparse_decode_steps_over_the_cache(dtype, fmt):
                 assert torch.equal(torch.sort(scores[b, h][idx[b, h].long()], descending=True).values, want)
                 rows = union[h, :int(count[h])].long().cpu()
                 assert set(rows.tolist()) == set(idx[b, h].tolist()) | set(range(sink)) | set(range(length[b] - local, length[b]))
-                check_attention(out[0, h * G:(h + 1) * G], lse[0, h * G:(h + 1) * G], q[b, h * G:(h + 1) * G].cpu(), kd[b, rows, h], vd[b, rows, h], dt, True)
+                check_attention(out[0, h * G:(h + 1) * G], lse[0, h * G:(h + 1) * G], q[b, h * G:(h + 1) * G].cpu(), kd[b, rows, h], vd[b, rows, h], dt, dtype == "f16")
 
 
 def test_centre_selection_over_the_cache():

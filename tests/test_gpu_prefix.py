@@ -42,7 +42,7 @@ def _check(out, lse, q, pre, suf, length, G, dtype, fmt):
             n = min(max(length[b], 0), suf[0].shape[1]) if suf else 0
             k, v = (torch.cat([pre[i][0, :, h] if pre else none, suf[i][b, :n, h] if suf else none]) for i in range(2))
             qs = slice(h * G, (h + 1) * G)
-            check_attention(out[b, qs], None if lse is None else lse[b, qs], q[b, qs], k, v, out.dtype, fmt != "16bit" or dtype == "f16")
+            check_attention(out[b, qs], None if lse is None else lse[b, qs], q[b, qs], k, v, out.dtype, fmt == "16bit" or dtype == "f16")
 
 
 @pytest.mark.parametrize("dtype,fmt", KINDS)
@@ -62,6 +62,44 @@ def test_prefix(dtype, fmt, B, H, G, P, S, layout):
         for splits in (1, 3):
             out, lse = ops.prefix_decode(q.cuda(), pre, suf, SCALE, G, suffix_len=_i32(length), num_splits=splits, return_lse=True)
             _check(out, lse, q, (kp, vp), (ks, vs), length, G, dtype, fmt)
+
+
+@pytest.mark.parametrize("dtype,fmt", KINDS)
+@pytest.mark.parametrize("B,H,G,P,S", [(3, 2, 4, 600, 20), (7, 1, 4, 700, 40), (12, 1, 4, 900, 33), (24, 1, 4, 1100, 9), (40, 1, 8, 1300, 270),
+                                       (130, 1, 1, 513, 1), (64, 1, 2, 384, 7)])
+def test_prefix_blocks_of_query_rows(dtype, fmt, B, H, G, P, S):
+    """Each form of the shared part (12, 28, 48, 96, 320, 130, 128 query rows of a head), several tiles of every wave."""
+    announce("prefix blocks %s %s B%d H%d G%d P%d S%d" % (dtype, fmt, B, H, G, P, S))
+    gen = torch.Generator().manual_seed(B * P + 1)
+    pre, kp, vp = _source(gen, (1, P, H, 128), dtype, fmt, "heads")
+    suf, ks, vs = _source(gen, (B, S, H, 128), dtype, fmt, "tokens")
+    q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype])
+    length = [(S, 0, 1, S // 2)[b % 4] for b in range(B)]
+    for splits in (0, 1, 2):
+        out, lse = ops.prefix_decode(q.cuda(), pre, suf, SCALE, G, suffix_len=_i32(length), num_splits=splits, return_lse=True)
+        _check(out, lse, q, (kp, vp), (ks, vs), length, G, dtype, fmt)
+
+
+@pytest.mark.parametrize("dtype,fmt", [k for k in KINDS if k[1] != "16bit"])
+@pytest.mark.parametrize("B", [2, 20, 40])
+def test_prefix_scales_far_apart(dtype, fmt, B):
+    """Value scales of a shared prefix that differ by 2^60, also between the tiles that share operands; NaN rows stay visible."""
+    H, G, P = 1, 8, 900
+    gen = torch.Generator().manual_seed(19)
+    pre, kp, vp = _source(gen, (1, P, H, 128), dtype, fmt, "heads")
+    far = torch.exp2(torch.randint(-50, 11, (1, P, H), generator=gen).float())
+    far[:, 300:600] = torch.exp2(torch.tensor(-60.0))
+    pre.v_scale.mul_(far.cuda())
+    vp = vp * far.double()[..., None]
+    q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype])
+    announce("prefix far scales %s %s B%d" % (dtype, fmt, B))
+    out, lse = ops.prefix_decode(q.cuda(), pre, None, SCALE, G, out_dtype=torch.bfloat16, return_lse=True)
+    _check(out, lse, q, (kp, vp), None, [0] * B, G, dtype, fmt)
+    pre.v_scale[0, 700] = math.nan
+    out, lse = ops.prefix_decode(q.cuda(), pre, None, SCALE, G, return_lse=True)
+    assert torch.isnan(out).all() and torch.isfinite(lse).all()
+    pre.k_scale[0, 5] = math.nan
+    assert torch.isnan(ops.prefix_decode(q.cuda(), pre, None, SCALE, G, return_lse=True)[1]).all()
 
 
 @pytest.mark.parametrize("dtype,fmt", KINDS)
@@ -86,7 +124,7 @@ def test_masked_places_hold_anything(dtype, fmt):
     """NaN and infinities in the rows behind a suffix's length change nothing."""
     B, H, G = 3, 2, 4
     gen = torch.Generator().manual_seed(7)
-    pre, _, _ = _source(gen, (1, 90, H, 128), dtype, fmt, "tokens")
+    pre, _, _ = _source(gen, (1, 490, H, 128), dtype, fmt, "tokens")
     suf, _, _ = _source(gen, (B, 70, H, 128), dtype, fmt, "heads")
     q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype]).cuda()
     length = [70, 0, 37]
@@ -139,17 +177,18 @@ def test_equals_attention_over_the_whole():
 
 
 @pytest.mark.parametrize("fmt", ["16bit", "int8"])
-def test_graph_replays(fmt):
+@pytest.mark.parametrize("B,G", [(5, 4), (19, 8)])
+def test_graph_replays(fmt, B, G):
     """Two captured graphs and eager calls in turn: every replay gives what an eager call gives."""
-    B, H, G = 5, 2, 4
+    H = 2
     gen = torch.Generator().manual_seed(23)
     pre, _, _ = _source(gen, (1, 2000, H, 128), "bf16", fmt, "tokens")
     suf, _, _ = _source(gen, (B, 100, H, 128), "bf16", fmt, "heads")
-    length = _i32([100, 0, 50, 1, 99])
+    length = _i32([(100, 0, 50, 1, 99)[b % 5] for b in range(B)])
     qs = [torch.randn((B, H * G, 128), generator=gen).bfloat16().cuda() for _ in range(2)]
     plans = [ops.PrefixDecodePlan(q, pre, suf, SCALE, G, suffix_len=length, return_lse=True) for q in qs]
     graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
-    announce("prefix graphs %s" % fmt)
+    announce("prefix graphs %s B%d" % (fmt, B))
     torch.cuda.synchronize()
     for g, p in zip(graphs, plans):
         with torch.cuda.graph(g):

@@ -17,6 +17,7 @@ bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 
 
 constexpr int64_t kMaxExtent = 1ll << 46;      // elements that a stride may span: more than any memory, and no sum of offsets passes 64 bits
 constexpr int64_t kMaxItems = 0x7fffffff;      // workgroups of a launch, partials of a call
+constexpr int64_t kMaxRows = 0x7fffffff - 1024;  // (positions of a tile behind the end still fit 32 bits)
 
 bool spans_ok(int64_t count, int64_t stride) { return stride >= 0 && (count <= 1 ? stride <= kMaxExtent : stride <= kMaxExtent / (count - 1)); }
 bool strides_ok(int64_t nb, int64_t nn, int64_t nh, int64_t b, int64_t n, int64_t h) { return spans_ok(nb, b) && spans_ok(nn, n) && spans_ok(nh, h); }
@@ -39,7 +40,7 @@ int check_cache(const tka_kv_cache& c, bool values, bool allow_16bit) {
   if (c.format != TKA_KV_E4M3 && c.format != TKA_KV_INT8 && !(allow_16bit && c.format == TKA_KV_16BIT)) return TKA_EUNSUPPORTED;
   if (c.head_dim != TKA_HEAD_DIM) return TKA_EUNSUPPORTED;
   if (c.batch < 1 || c.num_kv_heads < 1 || c.rows < 1) return TKA_EINVAL;
-  if (c.batch > 65535 || c.num_kv_heads > 65535 || c.rows > 0x7fffffffLL) return TKA_EUNSUPPORTED;
+  if (c.batch > 65535 || c.num_kv_heads > 65535 || c.rows > kMaxRows) return TKA_EUNSUPPORTED;
   if (!c.k || (values && !c.v)) return TKA_EINVAL;
   if (!strides_ok(c.batch, c.rows, c.num_kv_heads, c.stride_b, c.stride_n, c.stride_h)) return TKA_EINVAL;
   if (c.rows > 1 && c.stride_n < TKA_HEAD_DIM) return TKA_EINVAL;
@@ -215,6 +216,7 @@ int check_decode(const tka_kvq_flash_decode_args* a) {
   rc = check_out(a->out, a->out_dtype, a->out_stride_b, c.batch, c.num_kv_heads, a->group);
   if (rc != TKA_OK) return rc;
   if (a->num_splits < 0 || a->num_splits > TKA_MAX_SPLITS) return TKA_EINVAL;
+  if (a->idx_len > kMaxRows) return TKA_EUNSUPPORTED;
   if (a->kv_idx ? a->idx_len < 1 : (a->kv_count != nullptr || a->idx_len != 0)) return TKA_EINVAL;
   return partials_ok((int64_t)c.batch * c.num_kv_heads * a->group, plan_decode(a));
 }

@@ -56,9 +56,12 @@ __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x
   if constexpr (F16) return mfma_f16(a, b, c);
   else return mfma_bf16(a, b, c);
 }
+// (by value: __builtin_bit_cast of an element of a vector takes the vector's first element, whichever was named)
+__device__ __forceinline__ f16x2 as_f16(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
+__device__ __forceinline__ uint32_t as_bits(f16x2 x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const f16x2 v = {(_Float16)lo, (_Float16)hi};
-  return __builtin_bit_cast(uint32_t, v);
+  return as_bits(v);
 }
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -346,9 +349,7 @@ struct Rows {
           const float x = kQuantised<FMT> && !SCALED ? a * weight[2 * w] : a, y = kQuantised<FMT> && !SCALED ? b * weight[2 * w + 1] : b;
           pf[r][w] = pack_f16(x, y);
           if constexpr (kSplit) {
-            uint32_t hi = pf[r][w];
-            asm("" : "+v"(hi));   // (the compiler otherwise folds the conversions into mixed-precision multiply-adds and takes the first pair's rounded weights for all four)
-            const f16x2 h = __builtin_bit_cast(f16x2, hi);
+            const f16x2 h = as_f16(pf[r][w]);
             pf_lo[r][w] = pack_f16(x - (float)h[0], y - (float)h[1]);
           }
         } else {
@@ -826,8 +827,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       if constexpr (kScaled) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          even[w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, even[w]) * __builtin_bit_cast(f16x2, factor[w]));
-          odd[w] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, odd[w]) * __builtin_bit_cast(f16x2, factor[w]));
+          even[w] = as_bits(as_f16(even[w]) * as_f16(factor[w]));
+          odd[w] = as_bits(as_f16(odd[w]) * as_f16(factor[w]));
         }
       }
       sh.of.frag[wave][8 + 2 * D][lane] = even;
