@@ -9,7 +9,8 @@
  *
  * The conventions are those of topk_attn.h: device pointers owned by the caller, asynchronous on `stream`, no
  * allocation, tka_status returned, every check before the first HIP call, reserved fields zero, 64-bit offsets.
- * `stream` and all pointers belong to the device that is current when the call is made.
+ * `stream` and all pointers belong to the device that is current when the call is made.  A call whose rows would take
+ * more than 2^32 - 1 threads gives TKA_EUNSUPPORTED.
  *
  * An 8-bit row.  The 128 elements x of one (batch entry, token, KV head) are held as 128 one-byte codes and one fp32
  * scale and stand for code * scale.  Let A = max |x|.

@@ -219,3 +219,44 @@ def test_offsets_beyond_32_bits():
     announce("prefix far offsets")
     out, lse = ops.prefix_decode(q.cuda(), tuple(far), None, SCALE, 4, return_lse=True)
     _check(out, lse, q, (k.double(), v.double()), None, [0, 0], 4, "f16", "16bit")
+
+
+BLOCKS = [(4, 4), (8, 4), (16, 4), (16, 8), (40, 8)]      # query rows of a head: 16, 32, 64, 128 and more
+
+
+@pytest.mark.parametrize("fmt", ["16bit", "e4m3", "int8"])
+@pytest.mark.parametrize("B,G", BLOCKS)
+def test_a_bad_query_stays_alone(fmt, B, G):
+    """A query with a NaN or an infinity makes its own row NaN and no other row of its block."""
+    gen = torch.Generator().manual_seed(31)
+    pre, kp, vp = _source(gen, (1, 400, 1, 128), "bf16", fmt, "heads")
+    suf, ks, vs = _source(gen, (B, 20, 1, 128), "bf16", fmt, "tokens")
+    q = torch.randn((B, G, 128), generator=gen).bfloat16()
+    announce("prefix bad query %s B%d G%d" % (fmt, B, G))
+    clean, clean_lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), suf, SCALE, G, return_lse=True)
+    _check(clean, clean_lse, q, (kp, vp), (ks, vs), [20] * B, G, "bf16", fmt)
+    bad = q.clone()
+    bad[1, 2, 5], bad[B - 1, G - 1, 100] = math.nan, math.inf
+    out, lse = ops.prefix_decode(bad.cuda(), _as_prefix(pre), suf, SCALE, G, return_lse=True)
+    hit = torch.zeros((B, G), dtype=torch.bool)
+    hit[1, 2] = hit[B - 1, G - 1] = True
+    hit = hit.cuda()
+    assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+    _check(torch.where(hit[..., None], clean, out), torch.where(hit, clean_lse, lse), q, (kp, vp), (ks, vs), [20] * B, G, "bf16", fmt)
+
+
+@pytest.mark.parametrize("dtype,fmt", KINDS)
+@pytest.mark.parametrize("B,G", BLOCKS)
+def test_prefix_any_number_of_splits(dtype, fmt, B, G):
+    """One split, two and the most there may be; the scales of some value rows negative."""
+    P = 1500
+    gen = torch.Generator().manual_seed(37)
+    pre, kp, vp = _source(gen, (1, P, 1, 128), dtype, fmt, "heads")
+    if fmt != "16bit":
+        pre.v_scale[:, ::3] *= -1
+        vp[:, ::3] *= -1
+    q = torch.randn((B, G, 128), generator=gen).to(DTYPES[dtype])
+    announce("prefix splits %s %s B%d G%d" % (dtype, fmt, B, G))
+    for splits in (1, 2, 512):
+        out, lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), None, SCALE, G, num_splits=splits, return_lse=True)
+        _check(out, lse, q, (kp, vp), None, [0] * B, G, dtype, fmt)

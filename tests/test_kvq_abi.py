@@ -190,3 +190,29 @@ def test_ops_refuse_cpu_tensors():
         ops.QuantCache(codes, codes, scale, scale)
     with pytest.raises(ValueError):
         ops.prefix_decode(q, (k[0], k[0]), (k, k), 1.0)
+
+
+def test_launches_stay_within_the_limit():
+    """Calls whose rows would take more than 2^32 - 1 threads are refused before anything is launched."""
+    lib = L.lib()
+    a = _copy(L.KvqWriteArgs)      # 2^29 rows: 2^24 workgroups of 256 threads
+    a.cache.batch, a.cache.num_kv_heads, a.num_tokens, a.stride_b, a.stride_n, a.stride_h = 1, 1, 1 << 29, 0, 0, 0
+    assert lib.tka_kvq_write(C.byref(a)) == UNSUPPORTED
+    a = _scores()                  # 2^32 rows of a shared cache
+    a.cache.batch, a.cache.num_kv_heads, a.cache.rows, a.cache.stride_b, a.cache.scale_stride_b = 4096, 4, 1 << 18, 0, 0
+    assert lib.tka_kvq_scores(C.byref(a)) == UNSUPPORTED
+    for rows in (200, 1000):       # 2^23 query heads, one launch or two
+        a = _decode()
+        a.cache.batch, a.cache.num_kv_heads, a.cache.rows, a.group, a.cache.stride_b, a.cache.scale_stride_b = 32768, 256, rows, 1, 0, 0
+        a.q_stride_b = a.out_stride_b = 256 * 128
+        assert lib.tka_kvq_flash_decode(C.byref(a)) == UNSUPPORTED
+        a.cache.batch = 32767
+        assert lib.tka_kvq_flash_decode(C.byref(a)) == L.TKA_EWORKSPACE
+        a = _prefix()
+        a.prefix.rows, a.suffix.rows, a.suffix.batch, a.group = rows, 0, 32768, 1
+        a.prefix.num_kv_heads = a.suffix.num_kv_heads = 256
+        a.q_stride_b = a.out_stride_b = 256 * 128
+        assert lib.tka_prefix_decode(C.byref(a)) == (UNSUPPORTED if rows == 200 else L.TKA_EWORKSPACE)
+        a.suffix.batch, a.group = 32768, 4
+        a.q_stride_b = a.out_stride_b = 1024 * 128
+        assert lib.tka_prefix_decode(C.byref(a)) == UNSUPPORTED

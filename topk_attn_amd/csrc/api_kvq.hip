@@ -16,7 +16,8 @@ bool group_ok(int g) { return g == 1 || g == 2 || g == 4 || g == 8; }
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 constexpr int64_t kMaxExtent = 1ll << 46;      // elements that a stride may span: more than any memory, and no sum of offsets passes 64 bits
-constexpr int64_t kMaxItems = 0x7fffffff;      // workgroups of a launch, partials of a call
+constexpr int64_t kMaxItems = 0x7fffffff;      // rows of a call, partials of a call
+constexpr int64_t kMaxThreads = 0xffffffff;    // of a launch
 constexpr int64_t kMaxRows = 0x7fffffff - 1024;  // (positions of a tile behind the end still fit 32 bits)
 
 bool spans_ok(int64_t count, int64_t stride) { return stride >= 0 && (count <= 1 ? stride <= kMaxExtent : stride <= kMaxExtent / (count - 1)); }
@@ -84,7 +85,8 @@ int check_copy(const Args* a, bool write) {
   if (!strides_ok(c.batch, a->num_tokens, c.num_kv_heads, a->stride_b, a->stride_n, a->stride_h)) return TKA_EINVAL;
   if ((a->stride_b | a->stride_n | a->stride_h) & 7) return TKA_EINVAL;
   if (!aligned(a->k, 16) || !aligned(a->v, 16)) return TKA_EINVAL;
-  if ((int64_t)c.batch * c.num_kv_heads * a->num_tokens > kMaxItems) return TKA_EUNSUPPORTED;
+  const int64_t pairs = (int64_t)c.batch * c.num_kv_heads;
+  if (a->num_tokens > kMaxItems / pairs || copy_grid(pairs, a->num_tokens).workgroups > kMaxThreads / 256) return TKA_EUNSUPPORTED;
   if (write) {
     if (!disjoint(TKA_HEAD_DIM, c.batch, c.rows, c.num_kv_heads, c.stride_b, c.stride_n, c.stride_h) ||
         !disjoint(1, c.batch, c.rows, c.num_kv_heads, c.scale_stride_b, c.scale_stride_n, c.scale_stride_h))
@@ -145,7 +147,8 @@ int check_scores(const tka_kvq_scores_args* a) {
   rc = check_query(a->q, a->dtype, a->group, a->q_stride_b, a->cache.batch, a->cache.num_kv_heads);
   if (rc != TKA_OK) return rc;
   if (!a->out_scores || a->reserved0 != 0) return TKA_EINVAL;
-  if ((int64_t)a->cache.batch * a->cache.num_kv_heads * ((a->cache.rows + 255) / 256) > kMaxItems) return TKA_EUNSUPPORTED;
+  const int64_t segs = (int64_t)a->cache.batch * a->cache.num_kv_heads;
+  if ((a->cache.rows + kScoreTokens - 1) / kScoreTokens > kMaxThreads / 256 / segs) return TKA_EUNSUPPORTED;
   return TKA_OK;
 }
 
@@ -202,7 +205,13 @@ Plan plan_prefix(const tka_prefix_decode_args* a) {
   return p;
 }
 
-int partials_ok(int64_t rows, const Plan& p) { return rows * p.parts() <= kMaxItems ? TKA_OK : TKA_EUNSUPPORTED; }
+// The launches: a workgroup of up to 512 threads per item, then one of 256 per query row.
+int launches_ok(int64_t batch, int64_t heads, int group, const Plan& p) {
+  const int64_t segs = batch * heads, rows = segs * group;
+  if (rows * p.parts() > kMaxItems || rows > kMaxThreads / 256) return TKA_EUNSUPPORTED;
+  const int64_t items = p.row_tiles ? p.row_blocks * heads * p.shared_splits + segs * p.own_splits : segs;
+  return items <= kMaxThreads / 512 ? TKA_OK : TKA_EUNSUPPORTED;
+}
 
 int check_decode(const tka_kvq_flash_decode_args* a) {
   if (!a) return TKA_EINVAL;
@@ -218,7 +227,7 @@ int check_decode(const tka_kvq_flash_decode_args* a) {
   if (a->num_splits < 0 || a->num_splits > TKA_MAX_SPLITS) return TKA_EINVAL;
   if (a->idx_len > kMaxRows) return TKA_EUNSUPPORTED;
   if (a->kv_idx ? a->idx_len < 1 : (a->kv_count != nullptr || a->idx_len != 0)) return TKA_EINVAL;
-  return partials_ok((int64_t)c.batch * c.num_kv_heads * a->group, plan_decode(a));
+  return launches_ok(c.batch, c.num_kv_heads, a->group, plan_decode(a));
 }
 
 int check_prefix(const tka_prefix_decode_args* a) {
@@ -238,7 +247,7 @@ int check_prefix(const tka_prefix_decode_args* a) {
   rc = check_out(a->out, a->out_dtype, a->out_stride_b, suf.batch, suf.num_kv_heads, a->group);
   if (rc != TKA_OK) return rc;
   if (a->num_splits < 0 || a->num_splits > TKA_MAX_SPLITS / 2) return TKA_EINVAL;
-  return partials_ok((int64_t)suf.batch * suf.num_kv_heads * a->group, plan_prefix(a));
+  return launches_ok(suf.batch, suf.num_kv_heads, a->group, plan_prefix(a));
 }
 
 // The workspace: references and sums, then accumulators (nothing where one workgroup writes the result).

@@ -632,16 +632,16 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
     const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (kQuantised<FMT> ? rows.cap : 1.0f);   // (an empty wave holds zeros)
     if (r) __syncthreads();
     if (wave < kJoined) {
-    if (j == 0) {
-      sh.m[wave][n] = rows.m_ref[r];
-      sh.l[wave][n] = l;
-    }
+      if (j == 0) {
+        sh.m[wave][n] = rows.m_ref[r];
+        sh.l[wave][n] = l;
+      }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float* to = &sh.acc[wave][n][32 * j + 8 * i];
-      *(f32x4*)to = (f32x4){rows.acc[r][0][i], rows.acc[r][1][i], rows.acc[r][2][i], rows.acc[r][3][i]} * norm;
-      *(f32x4*)(to + 4) = (f32x4){rows.acc[r][4][i], rows.acc[r][5][i], rows.acc[r][6][i], rows.acc[r][7][i]} * norm;
-    }
+      for (int i = 0; i < 4; ++i) {
+        float* to = &sh.acc[wave][n][32 * j + 8 * i];
+        *(f32x4*)to = (f32x4){rows.acc[r][0][i], rows.acc[r][1][i], rows.acc[r][2][i], rows.acc[r][3][i]} * norm;
+        *(f32x4*)(to + 4) = (f32x4){rows.acc[r][4][i], rows.acc[r][5][i], rows.acc[r][6][i], rows.acc[r][7][i]} * norm;
+      }
     }
     __syncthreads();
     // sixteen threads a row, eight dims each

@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRowLanes = 8;                       // lanes of a row, 16 elements each
-constexpr int kRowsPerWg = kThreads / kRowLanes;   // 32
+static_assert(kCopyRows == kThreads / kRowLanes, "");
 
 // Code pairs / quads of one dword as fp32 numbers.
 template <int FMT>
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void kvq_read_kernel(KvqCopyParams p, uin
 // takes the pair i = x (x < 4) or 11 - x, so that distance 8 is the DPP half mirror (i(7 - x) = i(x) ^ 4) and 4 and 2 are quad
 // permutations: no exchange goes through the LDS crossbar, and the sums pair up as in the definition.
 constexpr int kScoreRound = 64;
-constexpr int kScoreTokens = (kThreads / kWave) * kScoreRound;   // tokens of a workgroup (512: 95 us where 256 take 92, 1024: 102)
+static_assert(kScoreTokens == (kThreads / kWave) * kScoreRound, "");
 
 __device__ __forceinline__ float sum8(float p) {   // over eight lanes; every lane ends with the sum
   p = p + dpp_f32<0x141>(p);   // row_half_mirror
@@ -260,36 +260,26 @@ int by_type(int dtype, int format, Launch launch) {
                                : launch(std::integral_constant<int, TKA_BF16>(), std::integral_constant<int, TKA_KV_INT8>());
 }
 
-// Tiles of 32 tokens of one head; calls of fewer tokens take several heads into a workgroup.
-uint32_t copy_grid(KvqCopyParams* p, uint32_t* token_tiles) {
-  int log2 = 0;
-  while (log2 < 5 && (1 << log2) < p->num_tokens) ++log2;
-  p->tile_log2 = log2;
-  *token_tiles = (uint32_t)(((int64_t)p->num_tokens + (1 << log2) - 1) >> log2);
-  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads, per_wg = kRowsPerWg >> log2;
-  return (uint32_t)(*token_tiles * ((pairs + per_wg - 1) / per_wg));
-}
-
 }  // namespace
 
 int launch_kvq_write(const KvqCopyParams& p0, int dtype, int format, hipStream_t stream) {
   KvqCopyParams p = p0;
-  uint32_t tiles;
-  const uint32_t grid = copy_grid(&p, &tiles);
+  const CopyGrid grid = copy_grid((int64_t)p.batch * p.num_kv_heads, p.num_tokens);
+  p.tile_log2 = grid.tile_log2;
   LaunchTimer timer("kvq_write", stream);
   return by_type(dtype, format, [&](auto dt, auto fmt) {
-    kvq_write_kernel<dt(), fmt()><<<grid, kThreads, 0, stream>>>(p, tiles);
+    kvq_write_kernel<dt(), fmt()><<<(uint32_t)grid.workgroups, kThreads, 0, stream>>>(p, (uint32_t)grid.token_tiles);
     return hip_status(hipGetLastError());
   });
 }
 
 int launch_kvq_read(const KvqCopyParams& p0, int dtype, int format, hipStream_t stream) {
   KvqCopyParams p = p0;
-  uint32_t tiles;
-  const uint32_t grid = copy_grid(&p, &tiles);
+  const CopyGrid grid = copy_grid((int64_t)p.batch * p.num_kv_heads, p.num_tokens);
+  p.tile_log2 = grid.tile_log2;
   LaunchTimer timer("kvq_read", stream);
   return by_type(dtype, format, [&](auto dt, auto fmt) {
-    kvq_read_kernel<dt(), fmt()><<<grid, kThreads, 0, stream>>>(p, tiles);
+    kvq_read_kernel<dt(), fmt()><<<(uint32_t)grid.workgroups, kThreads, 0, stream>>>(p, (uint32_t)grid.token_tiles);
     return hip_status(hipGetLastError());
   });
 }
