@@ -260,3 +260,47 @@ def test_prefix_any_number_of_splits(dtype, fmt, B, G):
     for splits in (1, 2, 512):
         out, lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), None, SCALE, G, num_splits=splits, return_lse=True)
         _check(out, lse, q, (kp, vp), None, [0] * B, G, dtype, fmt)
+
+
+@pytest.mark.parametrize("dtype,fmt", KINDS)
+@pytest.mark.parametrize("B,H,G,P,S", [(17, 16, 8, 300, 40), (65, 4, 2, 1100, 129), (130, 2, 1, 500, 1), (33, 8, 4, 290, 260)])
+def test_many_short_suffixes(dtype, fmt, B, H, G, P, S):
+    """More than 128 query rows of a head and 256 suffixes or more, of every length: empty ones, whole ones, and one that holds
+    NaN behind its end."""
+    announce("prefix many suffixes %s %s B%d H%d G%d P%d S%d" % (dtype, fmt, B, H, G, P, S))
+    gen = torch.Generator().manual_seed(P + S)
+    pre, kp, vp = _source(gen, (1, P, H, 128), dtype, fmt, "heads")
+    suf, ks, vs = _source(gen, (B, S, H, 128), dtype, fmt, "tokens")
+    length = [(S, 0, 1, S // 2, S - 1)[b % 5] for b in range(B)]
+    for b in range(B):
+        for x in (suf[0], suf[1]) if fmt == "16bit" else (suf.k_scale, suf.v_scale):
+            x[b, length[b]:] = math.nan
+    q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype])
+    for splits in (0, 1):
+        out, lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), suf, SCALE, G, suffix_len=_i32(length), num_splits=splits, return_lse=True)
+        some = [0, 1, 2, 3, B - 1]
+        _check(out[some], lse[some], q[some], (kp, vp), (ks[some], vs[some]), [length[b] for b in some], G, dtype, fmt)
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+def test_many_short_suffixes_in_a_graph():
+    """The form of many short suffixes captured before any eager call of its shape, replayed over changing queries and lengths."""
+    B, H, G, P, S = 33, 8, 8, 700, 50
+    gen = torch.Generator().manual_seed(41)
+    pre, _, _ = _source(gen, (1, P, H, 128), "bf16", "e4m3", "heads")
+    suf, _, _ = _source(gen, (B, S, H, 128), "bf16", "e4m3", "heads")
+    q = torch.randn((B, H * G, 128), generator=gen).bfloat16().cuda()
+    length = _i32([b % (S + 1) for b in range(B)])
+    plan = ops.PrefixDecodePlan(q, pre, suf, SCALE, G, suffix_len=length, return_lse=True)
+    graph = torch.cuda.CUDAGraph()
+    announce("prefix many suffixes graph")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        plan.run()
+    for step in range(4):
+        q.copy_(torch.randn(q.shape, generator=gen))
+        graph.replay()
+        out, lse = ops.prefix_decode(q, pre, suf, SCALE, G, suffix_len=length, return_lse=True)
+        torch.cuda.synchronize()
+        assert torch.equal(plan.out, out) and torch.equal(plan.lse, lse)
+        length.sub_(7).clamp_(min=0)

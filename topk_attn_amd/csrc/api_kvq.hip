@@ -167,7 +167,9 @@ int log2_of(int group) { return group == 8 ? 3 : group >> 1; }
 struct Plan {
   int row_tiles, row_blocks;
   int shared_splits, shared_tps, own_splits, own_tps;
-  int parts() const { return row_tiles ? shared_splits + own_splits : 1; }
+  bool join_own;   // the own rows are attended to by the launch that joins the partials of the shared ones
+  int parts() const { return row_tiles ? shared_splits + (join_own ? 0 : own_splits) : 1; }
+  bool to_workspace() const { return parts() > 1 || join_own; }
 };
 
 // Calls of up to this many positions per (entry, head) take one launch of one workgroup each instead of a split and a join
@@ -175,7 +177,7 @@ struct Plan {
 constexpr int64_t kSoloLen = 256;
 
 Plan plan_decode(const tka_kvq_flash_decode_args* a) {
-  Plan p = {1, 0, 0, 0, 0, 0};
+  Plan p = {1, 0, 0, 0, 0, 0, false};
   const int64_t segs = (int64_t)a->cache.batch * a->cache.num_kv_heads;
   const int64_t len = a->kv_idx ? a->idx_len : a->cache.rows;
   if (!a->num_splits && len <= kSoloLen) {
@@ -188,7 +190,7 @@ Plan plan_decode(const tka_kvq_flash_decode_args* a) {
 }
 
 Plan plan_prefix(const tka_prefix_decode_args* a) {
-  Plan p = {1, 0, 0, 0, 0, 0};
+  Plan p = {1, 0, 0, 0, 0, 0, false};
   const int64_t heads = a->prefix.num_kv_heads, batch = a->suffix.batch, query_rows = batch * a->group;
   if (!a->num_splits && a->prefix.rows + a->suffix.rows <= kSoloLen) {
     p.row_tiles = 0;
@@ -201,7 +203,13 @@ Plan plan_prefix(const tka_prefix_decode_args* a) {
     p.row_blocks = (int)((query_rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     cut(a->prefix.rows, a->num_splits ? a->num_splits : (p.row_tiles == 4 || p.row_tiles == 16 ? 256 : 512) / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
   }
-  if (a->suffix.rows) cut(a->suffix.rows, 256 / (heads * batch), TKA_MAX_SPLITS / 2, &p.own_splits, &p.own_tps);
+  // The blocks of 256 query rows leave no room on a CU beside them (LDS), so that the suffixes would come after them, one workgroup
+  // a CU.  Many short suffixes are attended to by the launch that joins the partials instead, three workgroups a CU: (batch x heads
+  // x group, prefix, suffix) 64 x 8 x 8, 32768, 256 of e4m3 114 -> 108 us; 64 x 8 x 8, 4096, 1000 64 -> 55; 33 x 16 x 4, 4096, 33 of
+  // int8 35 -> 28; 32 x 8 x 8, 16384, 256 49 -> 47.  Fewer workgroups or longer suffixes lose: 64 x 2 x 8, 16384, 1000 41 -> 47;
+  // 32 x 8 x 8, 8192, 4000 89 -> 99; so do the smaller blocks: 16 x 8 x 4, 32768, 500 42 -> 45.
+  p.join_own = p.row_tiles == 16 && a->suffix.rows && a->suffix.rows <= 1024 && heads * batch >= 256;
+  if (a->suffix.rows) cut(a->suffix.rows, p.join_own ? 1 : 256 / (heads * batch), TKA_MAX_SPLITS / 2, &p.own_splits, &p.own_tps);
   return p;
 }
 
@@ -209,7 +217,7 @@ Plan plan_prefix(const tka_prefix_decode_args* a) {
 int launches_ok(int64_t batch, int64_t heads, int group, const Plan& p) {
   const int64_t segs = batch * heads, rows = segs * group;
   if (rows * p.parts() > kMaxItems || rows > kMaxThreads / 256) return TKA_EUNSUPPORTED;
-  const int64_t items = p.row_tiles ? p.row_blocks * heads * p.shared_splits + segs * p.own_splits : segs;
+  const int64_t items = p.row_tiles ? p.row_blocks * heads * p.shared_splits + segs * p.own_splits : segs;   // (at least those of each launch)
   return items <= kMaxThreads / 512 ? TKA_OK : TKA_EUNSUPPORTED;
 }
 
@@ -252,7 +260,7 @@ int check_prefix(const tka_prefix_decode_args* a) {
 
 // The workspace: references and sums, then accumulators (nothing where one workgroup writes the result).
 size_t partial_bytes(int64_t segs, int group, const Plan& p) {
-  const size_t parts = p.parts() > 1 ? (size_t)segs * group * (size_t)p.parts() : 0;
+  const size_t parts = p.to_workspace() ? (size_t)segs * group * (size_t)p.parts() : 0;
   return align_up(parts * 2 * sizeof(float), 256) + align_up(parts * TKA_HEAD_DIM * sizeof(float), 256) + 256;   // (never 0, which stands for a refused call)
 }
 
@@ -260,15 +268,16 @@ int run_attend(KvAttendParams p, const Plan& plan, int dtype, int format, void* 
   p.row_blocks = plan.row_blocks;
   p.shared_splits = plan.shared_splits;
   p.shared_tps = plan.shared_tps;
-  p.own_splits = plan.own_splits;
+  p.own_splits = plan.join_own ? 0 : plan.own_splits;
   p.own_tps = plan.own_tps;
   p.num_splits = plan.parts();
+  p.to_workspace = plan.to_workspace();
   const size_t parts = (size_t)p.batch * p.num_kv_heads * ((size_t)p.num_splits << p.group_log2);
   p.part_ml = (f32x2*)workspace;
   p.part_acc = (float*)((unsigned char*)workspace + align_up(parts * 2 * sizeof(float), 256));
   const int rc = launch_kv_attend(p, dtype, format, plan.row_tiles, stream);
-  if (rc != TKA_OK || p.num_splits == 1) return rc;
-  return launch_kv_combine(p, stream);
+  if (rc != TKA_OK || !p.to_workspace) return rc;
+  return plan.join_own ? launch_kv_attend_join(p, dtype, format, stream) : launch_kv_combine(p, stream);
 }
 
 }  // namespace

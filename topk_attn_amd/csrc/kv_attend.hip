@@ -463,7 +463,7 @@ __device__ __forceinline__ void clear_masked(uint32_t masked, VRow<FMT> (&vr)[8]
 // Partial of one split (a join follows) or the finished row, dims d0 .. d0 + 7.
 template <bool F16>
 __device__ __forceinline__ void store_result(const KvAttendParams& p, int b, int hq, int slot, int d0, const f32x4& lo, const f32x4& hi, float M, float L) {
-  if (p.num_splits > 1) {
+  if (p.to_workspace) {
     const int64_t at = ((((int64_t)b * p.num_kv_heads) << p.group_log2) + hq) * p.num_splits + slot;
     f32x4* to = (f32x4*)(p.part_acc + at * kHeadDim + d0);
     to[0] = lo;
@@ -475,7 +475,58 @@ __device__ __forceinline__ void store_result(const KvAttendParams& p, int b, int
   }
 }
 
-template <int DT, int FMT, int RT, bool INDEXED, int WAVES>
+// Joins what 256 threads hold of a workgroup's own rows (thread: dims d0 .. d0+7 of query row `row`, reference M in base 2, sum L;
+// part `part` of `parts` for each row) with the partials of the shared rows, and writes the rows.
+__device__ __forceinline__ void join_shared(const KvAttendParams& p, int b, int hq, int d0, int slot, int part, int parts, f32x4 lo, f32x4 hi, float M,
+                                            float L, float (&sh)[16][kLdsRow]) {
+  const int S = p.num_splits, x = threadIdx.x & 15;
+  const int64_t at = ((((int64_t)b * p.num_kv_heads) << p.group_log2) + hq) * S;
+  const f32x2* ml = p.part_ml + at;
+  const f32x4* pa = (const f32x4*)(p.part_acc + at * kHeadDim + d0);
+  float top = M;
+  for (int s = x; s < S; s += 16) top = fmaxf(top, ml[s][0]);
+#pragma unroll
+  for (int y = 8; y >= 1; y >>= 1) top = fmaxf(top, __shfl_xor(top, y, 64));
+  float sum = 0.0f;
+  for (int s = x; s < S; s += 16) sum += ml[s][1] * __builtin_amdgcn_exp2f(ml[s][0] - top);
+#pragma unroll
+  for (int y = 8; y >= 1; y >>= 1) sum += __shfl_xor(sum, y, 64);
+  const float own = L * __builtin_amdgcn_exp2f(M - top);
+  sum += own;
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  lo *= part ? 0.0f : own * inv;
+  hi *= part ? 0.0f : own * inv;
+  for (int s0 = part; s0 < S; s0 += 4 * parts) {
+    f32x4 a[4], c[4];
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * parts < S ? s0 + u * parts : s0;
+      a[u] = pa[(int64_t)s * (kHeadDim / 4)];
+      c[u] = pa[(int64_t)s * (kHeadDim / 4) + 1];
+      w[u] = ml[s][1] * __builtin_amdgcn_exp2f(ml[s][0] - top) * inv;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s0 + u * parts < S) {
+        lo += a[u] * w[u];
+        hi += c[u] * w[u];
+      }
+  }
+  __syncthreads();   // (the own rows have been read)
+  *(f32x4*)&sh[slot][d0] = lo;
+  *(f32x4*)&sh[slot][d0 + 4] = hi;
+  __syncthreads();
+  if (part) return;
+  for (int y = 1; y < parts; ++y) {
+    lo += *(const f32x4*)&sh[slot + (y << p.group_log2)][d0];
+    hi += *(const f32x4*)&sh[slot + (y << p.group_log2)][d0 + 4];
+  }
+  store_row(p, b, hq, d0, lo, hi, top, sum, 0.0f);
+}
+
+// JOIN: the workgroup then joins its rows with the partials of the shared source and writes them.
+template <int DT, int FMT, int RT, bool INDEXED, int WAVES, bool JOIN = false>
 __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem& item, AttendLds& sh, int32_t* sh_ids) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -644,24 +695,31 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
       }
     }
     __syncthreads();
-    // sixteen threads a row, eight dims each
-    const int row = item.row0 + 16 * r + (tid >> 4), d0 = 8 * (tid & 15);
+    // sixteen threads a row, eight dims each (JOIN: all 256 share the `group` rows)
+    const int slot = JOIN ? (tid >> 4) & (group - 1) : tid >> 4, d0 = 8 * (tid & 15);
+    const int row = item.row0 + 16 * r + slot;
     if (tid < 16 * 16 && row < item.row_end) {
       float M = kNoReference, w[kJoined], L = 0.0f;   // w: l 2^(m - M) of the waves
 #pragma unroll
-      for (int x = 0; x < kJoined; ++x) M = fmaxf(M, sh.m[x][tid >> 4]);
+      for (int x = 0; x < kJoined; ++x) M = fmaxf(M, sh.m[x][slot]);
       f32x4 lo = (f32x4){0.f, 0.f, 0.f, 0.f}, hi = lo;
 #pragma unroll
       for (int x = 0; x < kJoined; ++x) {
-        w[x] = sh.l[x][tid >> 4] * __builtin_amdgcn_exp2f(sh.m[x][tid >> 4] - M);   // (0 without rows)
+        w[x] = sh.l[x][slot] * __builtin_amdgcn_exp2f(sh.m[x][slot] - M);   // (0 without rows)
         L += w[x];
       }
       const bool some = L > 0.0f || L != L;
       const float inv = some ? 1.0f / L : 0.0f;
 #pragma unroll
       for (int x = 0; x < kJoined; ++x) {
-        lo += *(const f32x4*)&sh.acc[x][tid >> 4][d0] * (w[x] * inv);
-        hi += *(const f32x4*)&sh.acc[x][tid >> 4][d0 + 4] * (w[x] * inv);
+        lo += *(const f32x4*)&sh.acc[x][slot][d0] * (w[x] * inv);
+        hi += *(const f32x4*)&sh.acc[x][slot][d0 + 4] * (w[x] * inv);
+      }
+      if constexpr (JOIN) {
+        static_assert(RT == 1 && WAVES == kJoined, "");
+        join_shared(p, item.b0, item.h * group + slot, d0, tid >> 4, tid >> 4 >> p.group_log2, 16 >> p.group_log2, lo, hi,
+                    M == kNoReference ? M : M - kWeightLog2<Rows<DT, FMT, RT>::kPF16>, L, sh.acc[0]);
+        return;
       }
       store_result<Rows<DT, FMT, RT>::kPF16>(p, item.b0 + (row >> p.group_log2), item.h * group + (row & (group - 1)), item.slot, d0, lo, hi, M, L);
     }
@@ -916,6 +974,22 @@ __global__ __launch_bounds__(kSoloWaves * kWave, 2) void kv_attend_solo_kernel(K
   attend<DT, FMT, 1, INDEXED, kSoloWaves>(p, item, sh, sh_ids);
 }
 
+// The second launch of calls with many short suffixes behind blocks of 256 query rows: a workgroup attends to the suffix of an (entry,
+// head) and joins it with the partials of the prefix.
+template <int DT, int FMT>
+__global__ __launch_bounds__(kThreads, 3) void kv_attend_join_kernel(KvAttendParams p) {
+  __shared__ AttendLds sh;
+  AttendItem item;
+  item.two = false;
+  item.b0 = (int)(blockIdx.x / (uint32_t)p.num_kv_heads);
+  item.h = (int)(blockIdx.x % (uint32_t)p.num_kv_heads);
+  item.row0 = 0;
+  item.row_end = 1 << p.group_log2;
+  item.slot = 0;
+  take_own<false>(p, 0, item.b0, item.h, &item.first);
+  attend<DT, FMT, 1, false, kWaves, true>(p, item, sh, nullptr);
+}
+
 // One workgroup per query row: 32 lanes hold the 128 dims, eight groups of them take every eighth split.  A row whose sum is
 // NaN stays NaN (an empty split holds zeros, so nothing has to be skipped); one without any key gets zeros and -infinity.
 constexpr int kCombineGroups = kThreads / 32;
@@ -1014,6 +1088,24 @@ int launch_format(const KvAttendParams& p, int format, int row_tiles, hipStream_
 int launch_kv_attend(const KvAttendParams& p, int dtype, int format, int row_tiles, hipStream_t stream) {
   LaunchTimer timer(p.shared_splits ? "prefix_attend" : (p.kv_idx ? "kvq_attend_indexed" : "kvq_attend_dense"), stream);
   return dtype == TKA_F16 ? launch_format<TKA_F16>(p, format, row_tiles, stream) : launch_format<TKA_BF16>(p, format, row_tiles, stream);
+}
+
+namespace {
+template <int DT>
+int launch_join_format(const KvAttendParams& p, int format, hipStream_t stream) {
+  const uint32_t grid = (uint32_t)(p.batch * p.num_kv_heads);
+  switch (format) {
+    case TKA_KV_16BIT: kv_attend_join_kernel<DT, TKA_KV_16BIT><<<grid, kThreads, 0, stream>>>(p); break;
+    case TKA_KV_E4M3: kv_attend_join_kernel<DT, TKA_KV_E4M3><<<grid, kThreads, 0, stream>>>(p); break;
+    default: kv_attend_join_kernel<DT, TKA_KV_INT8><<<grid, kThreads, 0, stream>>>(p); break;
+  }
+  return hip_status(hipGetLastError());
+}
+}  // namespace
+
+int launch_kv_attend_join(const KvAttendParams& p, int dtype, int format, hipStream_t stream) {
+  LaunchTimer timer("prefix_suffix_join", stream);
+  return dtype == TKA_F16 ? launch_join_format<TKA_F16>(p, format, stream) : launch_join_format<TKA_BF16>(p, format, stream);
 }
 
 int launch_kv_combine(const KvAttendParams& p, hipStream_t stream) {

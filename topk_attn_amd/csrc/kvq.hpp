@@ -76,6 +76,7 @@ struct KvAttendParams {
   const int32_t* kv_count;  // [batch][num_kv_heads] or nullptr
   int idx_len;
   int num_splits;           // partials per query row: shared_splits + own_splits
+  int to_workspace;         // the launch writes partials (0: finished rows)
   f32x2* part_ml;           // [rows][num_splits] reference (base 2) and sum of the weights
   float* part_acc;          // [rows][num_splits][128], normalised
   void* out;
@@ -87,6 +88,9 @@ struct KvAttendParams {
 constexpr int kAttendTile = 32;   // tokens of a wave's tile
 // row_tiles: RT of the shared source; 0 = the short form, one workgroup per (entry, head) and one split of each source.
 int launch_kv_attend(const KvAttendParams& p, int dtype, int format, int row_tiles, hipStream_t stream);
+
+// The own rows (one workgroup per entry and head, whatever own_splits says) joined with num_splits partials of the shared ones.
+int launch_kv_attend_join(const KvAttendParams& p, int dtype, int format, hipStream_t stream);
 
 // Joins the partials of the query rows and writes p.out / p.out_lse (num_splits > 1).
 int launch_kv_combine(const KvAttendParams& p, hipStream_t stream);
