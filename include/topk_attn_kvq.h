@@ -162,6 +162,10 @@ typedef struct tka_prefix_decode_args {
 size_t tka_prefix_decode_workspace_bytes(const tka_prefix_decode_args* args);
 int tka_prefix_decode(const tka_prefix_decode_args* args);
 
+/* Testing hook (process-wide): tka_prefix_decode takes 16 * row_tiles query rows (1, 2, 4, 8, 16; 16-bit rows: up to 4) with each
+ * tile of the prefix in place of the number it would choose, 0 = choose.  Results stay within the same error bounds. */
+int tka_kvq_test_row_tiles(int32_t row_tiles);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from kvq_util import CODES, DTYPES, SCALE, check_attention, laid, random_cache
-from topk_attn_amd import ops
+from topk_attn_amd import _lib as L, ops
 from util import announce
 
 pytestmark = pytest.mark.gpu
@@ -304,3 +304,62 @@ def test_many_short_suffixes_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(plan.out, out) and torch.equal(plan.lse, lse)
         length.sub_(7).clamp_(min=0)
+
+
+@pytest.fixture(params=[1, 2, 4, 8, 16])
+def row_tiles(request):
+    """Blocks of 16 times as many query rows, whatever the call would choose."""
+    assert L.lib().tka_kvq_test_row_tiles(request.param) == 0
+    yield request.param
+    assert L.lib().tka_kvq_test_row_tiles(0) == 0
+
+
+def _kinds_of(row_tiles):
+    return [(d, f) for d, f in KINDS if f != "16bit" or row_tiles <= 4]
+
+
+@pytest.mark.parametrize("B,H,G,P,S,layout", [(1, 1, 1, 1, 1, "tokens"), (5, 2, 4, 31, 3, "heads"), (9, 1, 8, 161, 40, "gaps"), (19, 2, 8, 700, 33, "heads"),
+                                              (40, 1, 8, 1301, 270, "tokens"), (65, 4, 4, 260, 30, "heads")])
+def test_every_block_size(row_tiles, B, H, G, P, S, layout):
+    """Blocks larger than the call, several blocks with a last one that is cut, prefixes shorter than a tile and cut ones."""
+    for dtype, fmt in _kinds_of(row_tiles):
+        announce("prefix blocks of %d: %s %s B%d H%d G%d P%d S%d %s" % (16 * row_tiles, dtype, fmt, B, H, G, P, S, layout))
+        gen = torch.Generator().manual_seed(B + P)
+        pre, kp, vp = _source(gen, (1, P, H, 128), dtype, fmt, layout)
+        suf, ks, vs = _source(gen, (B, S, H, 128), dtype, fmt, layout)
+        q = torch.randn((B, H * G, 128), generator=gen).to(DTYPES[dtype])
+        length = [(S, 0, 1, S // 2, S + 3)[b % 5] for b in range(B)]
+        out, lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), suf, SCALE, G, suffix_len=_i32(length), return_lse=True)
+        _check(out, lse, q, (kp, vp), (ks, vs), length, G, dtype, fmt)
+
+
+def test_every_block_size_where_it_can_go_wrong(row_tiles):
+    """The cases of the tests above with this block size: scales far apart, places that are masked, bad queries, any number of
+    splits, prefix or suffix alone, many short suffixes, replays."""
+    for dtype, fmt in _kinds_of(row_tiles):
+        if fmt != "16bit":
+            test_prefix_scales_far_apart(dtype, fmt, 20)
+        test_masked_places_hold_anything(dtype, fmt)
+        test_prefix_alone_and_suffix_alone(dtype, fmt)
+        test_prefix_any_number_of_splits(dtype, fmt, 40, 8)
+        test_many_short_suffixes(dtype, fmt, 33, 8, 4, 290, 260)
+        if dtype == "bf16":
+            test_a_bad_query_stays_alone(fmt, 19, 8)
+    for dtype in DTYPES:
+        test_extreme_16bit_rows(dtype)
+    test_graph_replays("int8", 19, 8)
+    test_many_short_suffixes_in_a_graph()
+
+
+@pytest.mark.parametrize("fmt,B,G,P", [("16bit", 3, 8, 40000), ("16bit", 40, 8, 60000), ("e4m3", 6, 8, 60000), ("int8", 40, 4, 200000), ("e4m3", 64, 8, 60000)])
+def test_the_blocks_that_long_prefixes_choose(fmt, B, G, P):
+    """Sizes at which the call itself takes blocks of 32, 64, 128 and 256 query rows; the output of a few entries is checked."""
+    announce("prefix long %s B%d G%d P%d" % (fmt, B, G, P))
+    gen = torch.Generator().manual_seed(P)
+    pre, kp, vp = _source(gen, (1, P, 1, 128), "bf16", fmt, "heads")
+    suf, ks, vs = _source(gen, (B, 40, 1, 128), "bf16", fmt, "heads")
+    q = torch.randn((B, G, 128), generator=gen).bfloat16()
+    out, lse = ops.prefix_decode(q.cuda(), _as_prefix(pre), suf, SCALE, G, return_lse=True)
+    some = [0, B // 2, B - 1]
+    _check(out[some], lse[some], q[some], (kp, vp), (ks[some], vs[some]), [40] * 3, G, "bf16", fmt)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()

@@ -216,3 +216,9 @@ def test_launches_stay_within_the_limit():
         a.suffix.batch, a.group = 32768, 4
         a.q_stride_b = a.out_stride_b = 1024 * 128
         assert lib.tka_prefix_decode(C.byref(a)) == UNSUPPORTED
+
+
+def test_the_hook_is_checked():
+    for n in (-1, 3, 5, 32):
+        assert L.lib().tka_kvq_test_row_tiles(n) == INVALID
+    assert L.lib().tka_kvq_test_row_tiles(0) == 0

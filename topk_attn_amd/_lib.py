@@ -179,6 +179,7 @@ KVQ_PROTOTYPES = {
     "tka_kvq_flash_decode": (C.c_int, [C.POINTER(KvqFlashDecodeArgs)]),
     "tka_prefix_decode_workspace_bytes": (_sz, [C.POINTER(PrefixDecodeArgs)]),
     "tka_prefix_decode": (C.c_int, [C.POINTER(PrefixDecodeArgs)]),
+    "tka_kvq_test_row_tiles": (C.c_int, [C.c_int32]),
 }
 
 _lib = None

@@ -3,6 +3,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <utility>
 
 #include "kvq.hpp"
@@ -189,17 +190,43 @@ Plan plan_decode(const tka_kvq_flash_decode_args* a) {
   return p;
 }
 
+// Query rows of a head that a workgroup takes with each tile of the prefix, in sixteens.  More of them save reads of the rows (of the
+// L2 and the memory-side cache: the blocks of a head run side by side) and conversions, fewer start and end sooner and leave the
+// CU to more workgroups, so the rule goes by the size of the products, query rows x heads x positions.  Times by sixteens 1 / 2 / 4 /
+// 8 / 16 in us, suffixes of 100:
+//   16 x 8 x 4 (64 rows), 1000 positions    16 bit  0.5 M   10.7 / 11.0 / 16.3 / 13.4 / 13.9
+//   10 x 8 x 4 (40), 8192                   int8    2.6 M   16.8 / 17.5 / 19.5 / 20.3 / 21.3
+//   16 x 8 x 4, 8192                        16 bit  4.2 M   23.2 / 21.1 / 24.0 / 27.0 / 26.5
+//   32 x 8 x 4 (128), 8192                  16 bit  8.4 M   33.8 / 26.1 / 27.3 / 35.6 / 31.6
+//   16 x 8 x 4, 32768                       16 bit   17 M   66.6 / 47.4 / 41.4 / 55.5 / 59.1
+//   32 x 8 x 4, 16384                       e4m3     17 M   38.6 / 30.0 / 32.8 / 34.9 / 33.9
+//   64 x 8 x 8 (512), 8192                  e4m3     34 M      - / 49.2 / 52.6 / 47.2 / 43.8
+//   32 x 8 x 4, 65536                       int8     67 M      - / 84.2 / 81.1 / 73.5 / 76.9
+//   64 x 8 x 8, 32768                       16 bit  134 M      -  / 206 /  130 /  129 /  131
+//   64 x 8 x 8, 32768                       e4m3    134 M      -  / 133 /  135 /  107 /  105
+int prefix_row_tiles(int64_t query_rows, int64_t positions, bool wide16) {
+  const int64_t work = query_rows * positions;
+  if (query_rows <= 16 || work <= 5 << 19) return 1;
+  if (query_rows <= 32 || work <= (wide16 ? 9 << 20 : 28 << 20)) return 2;
+  if (wide16 || query_rows <= 64) return 4;   // (16-bit rows have no conversion to share: blocks of 128 and 256 do not win)
+  return query_rows <= 128 ? 8 : 16;
+}
+
+std::atomic<int> g_row_tiles{0};   // tka_kvq_test_row_tiles
+
 Plan plan_prefix(const tka_prefix_decode_args* a) {
   Plan p = {1, 0, 0, 0, 0, 0, false};
   const int64_t heads = a->prefix.num_kv_heads, batch = a->suffix.batch, query_rows = batch * a->group;
-  if (!a->num_splits && a->prefix.rows + a->suffix.rows <= kSoloLen) {
+  const int hook = g_row_tiles.load(std::memory_order_relaxed);
+  if (!a->num_splits && !hook && a->prefix.rows + a->suffix.rows <= kSoloLen) {
     p.row_tiles = 0;
     if (a->prefix.rows) cut(a->prefix.rows, 1, 1, &p.shared_splits, &p.shared_tps);
     if (a->suffix.rows) cut(a->suffix.rows, 1, 1, &p.own_splits, &p.own_tps);
     return p;
   }
   if (a->prefix.rows) {
-    p.row_tiles = query_rows <= 16 ? 1 : (query_rows <= 32 ? 2 : query_rows <= 64 ? 4 : (query_rows <= 128 ? 8 : 16));
+    const bool wide16 = a->prefix.format == TKA_KV_16BIT;
+    p.row_tiles = hook ? (wide16 ? std::min(hook, 4) : hook) : prefix_row_tiles(query_rows, heads * a->prefix.rows, wide16);
     p.row_blocks = (int)((query_rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     cut(a->prefix.rows, a->num_splits ? a->num_splits : (p.row_tiles == 4 || p.row_tiles == 16 ? 256 : 512) / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
   }
@@ -371,6 +398,12 @@ int tka_prefix_decode(const tka_prefix_decode_args* a) {
   p.out_dtype = a->out_dtype;
   p.scale_log2e = a->scale * 1.44269504088896340736f;
   return run_attend(p, plan_prefix(a), a->dtype, a->prefix.format, a->workspace, (hipStream_t)a->stream);
+}
+
+int tka_kvq_test_row_tiles(int32_t row_tiles) {
+  if (row_tiles != 0 && row_tiles != 1 && row_tiles != 2 && row_tiles != 4 && row_tiles != 8 && row_tiles != 16) return TKA_EINVAL;
+  g_row_tiles.store(row_tiles, std::memory_order_relaxed);
+  return TKA_OK;
 }
 
 }  // extern "C"

@@ -801,12 +801,13 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
 // their way meanwhile.
 template <int DT, int FMT, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAttendParams p) {
+  static_assert(kQuantised<FMT>, "");
   using State = Rows<DT, FMT, 2>;
   constexpr int kMacro = WAVES * kTile;
   // Value operands with their scales in them, over a power of two of the tile: exact in e4m3, where scales are powers of two
   // (but for what lies 2^-24 below the tile's largest), and off by half a step of fp16 twice in int8, which is left to the
   // weights where these are kept in two parts.  It saves a product for every weight.
-  constexpr bool kScaled = kQuantised<FMT> && (FMT == TKA_KV_E4M3 || !State::kSplit);
+  constexpr bool kScaled = FMT == TKA_KV_E4M3 || !State::kSplit;
   struct Operands {
     u32x4 frag[WAVES][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
     float ks[WAVES][kTile], vs[WAVES][kTile];
@@ -844,7 +845,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       dense.begin(from);
       dense.key_rows(it, start, kt);
       dense.template value_rows<false>(it, start, vr);
-      if constexpr (kQuantised<FMT>) scale = (lane < kTile ? it.ks : it.vs)[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
+      scale = (lane < kTile ? it.ks : it.vs)[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
     }
   };
   // the operands of the tile in the registers, from position `tile` on
@@ -852,7 +853,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
     const int token = lane & (kTile - 1);
     const bool cut = it.end - tile < kTile;
     const int start = tile_start(tile, it.end);
-    if constexpr (kQuantised<FMT>) hold<FMT>(kt, vr);
+    hold<FMT>(kt, vr);
     if (cut) clear_masked<FMT>(tile_mask(start, tile, it.end), vr);
     u32x4 factor;   // of the value rows: pairs of slots
     if constexpr (kScaled) {
@@ -868,7 +869,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       const u32x2 lo = *(const u32x2*)(held + 4 * j), hi = *(const u32x2*)(held + 16 + 4 * j);
       factor = (u32x4){lo[0], lo[1], hi[0], hi[1]};
       if (lane < kTile) sh.of.ks[wave][token] = scale * p.scale_log2e;
-    } else if constexpr (kQuantised<FMT>) {
+    } else {
       (lane < kTile ? sh.of.ks : sh.of.vs)[wave][token] = lane < kTile ? scale * p.scale_log2e : scale;
     }
 #pragma unroll
@@ -916,9 +917,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       float kf[8], vf[8], tile_scale = 0.0f;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        f32x4 a = (f32x4){p.scale_log2e, p.scale_log2e, p.scale_log2e, p.scale_log2e}, b = a;
-        if constexpr (kQuantised<FMT>) a = *(const f32x4*)&sh.of.ks[t][16 * x + 4 * j];
-        if constexpr (kQuantised<FMT> && !kScaled) b = *(const f32x4*)&sh.of.vs[t][16 * x + 4 * j];
+        const f32x4 a = *(const f32x4*)&sh.of.ks[t][16 * x + 4 * j], b = kScaled ? a : *(const f32x4*)&sh.of.vs[t][16 * x + 4 * j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           kf[4 * x + i] = a[i];
@@ -938,7 +937,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const float l = sum_over_quarters(rows.l_run[r]);
-    const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (kQuantised<FMT> ? rows.cap : 1.0f);
+    const float norm = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * rows.cap;
     const int row = row0 + 16 * r + n;
     if (row < row_end) {
 #pragma unroll
@@ -1064,12 +1063,15 @@ int launch_typed(const KvAttendParams& p, int row_tiles, hipStream_t stream) {
     kv_attend_kernel<DT, FMT, 1, false><<<grid, kThreads, 0, stream>>>(p);
   } else if (row_tiles == 2) {
     kv_attend_kernel<DT, FMT, 2, false><<<grid, kThreads, 0, stream>>>(p);
-  } else if (row_tiles == 8) {
-    kv_attend_wide_kernel<DT, FMT, 4><<<grid, 4 * kWave, 0, stream>>>(p);
-  } else if (row_tiles == 16) {
-    kv_attend_wide_kernel<DT, FMT, 8><<<grid, 8 * kWave, 0, stream>>>(p);
-  } else {
+  } else if (row_tiles == 4) {
     kv_attend_kernel<DT, FMT, 4, false><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    if constexpr (kQuantised<FMT>) {
+      if (row_tiles == 8) kv_attend_wide_kernel<DT, FMT, 4><<<grid, 4 * kWave, 0, stream>>>(p);
+      else kv_attend_wide_kernel<DT, FMT, 8><<<grid, 8 * kWave, 0, stream>>>(p);
+    } else {
+      return TKA_EUNSUPPORTED;
+    }
   }
   return hip_status(hipGetLastError());
 }
@@ -1095,9 +1097,9 @@ template <int DT>
 int launch_join_format(const KvAttendParams& p, int format, hipStream_t stream) {
   const uint32_t grid = (uint32_t)(p.batch * p.num_kv_heads);
   switch (format) {
-    case TKA_KV_16BIT: kv_attend_join_kernel<DT, TKA_KV_16BIT><<<grid, kThreads, 0, stream>>>(p); break;
     case TKA_KV_E4M3: kv_attend_join_kernel<DT, TKA_KV_E4M3><<<grid, kThreads, 0, stream>>>(p); break;
-    default: kv_attend_join_kernel<DT, TKA_KV_INT8><<<grid, kThreads, 0, stream>>>(p); break;
+    case TKA_KV_INT8: kv_attend_join_kernel<DT, TKA_KV_INT8><<<grid, kThreads, 0, stream>>>(p); break;
+    default: return TKA_EUNSUPPORTED;
   }
   return hip_status(hipGetLastError());
 }
