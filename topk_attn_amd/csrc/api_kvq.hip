@@ -177,6 +177,15 @@ struct Plan {
 // (one sequence, 8 heads, group 4: 6.4 against 7.9 us at 256 positions, 8.6 against 7.8 at 512; host-bound below).
 constexpr int64_t kSoloLen = 256;
 
+// Splits of each (entry, head) of a decode.  Two workgroups a CU read best (4 x 8 x 32768 rows of e4m3: 256 workgroups 61 us, 512 45, 768
+// 47, 1024 51), but between 256 and 448 pairs, which fill the CUs unevenly, four splits each (320 pairs x 8000 rows: 131 -> 112 us,
+// 384 pairs 139 -> 135; 512 pairs in one split 168, in four 176).  Short calls save the second launch with one split: 32 pairs x 300
+// rows 7.8 -> 7.2 us (600: 8.0 -> 10.3), 128 x 600 12.0 -> 10.5 (1200: 15.0 -> 18.3), 256 x 1200 19.7 -> 19.4 (2400: 30.9 -> 33.3).
+int64_t decode_splits(int64_t segs, int64_t len) {
+  if (len <= std::max<int64_t>(384, std::min<int64_t>(6 * segs, 1280))) return 1;
+  return segs > 256 && segs < 448 ? 4 : 512 / segs;
+}
+
 Plan plan_decode(const tka_kvq_flash_decode_args* a) {
   Plan p = {1, 0, 0, 0, 0, 0, false};
   const int64_t segs = (int64_t)a->cache.batch * a->cache.num_kv_heads;
@@ -186,7 +195,7 @@ Plan plan_decode(const tka_kvq_flash_decode_args* a) {
     cut(len, 1, 1, &p.own_splits, &p.own_tps);
     return p;
   }
-  cut(len, a->num_splits ? a->num_splits : 512 / segs, TKA_MAX_SPLITS, &p.own_splits, &p.own_tps);
+  cut(len, a->num_splits ? a->num_splits : decode_splits(segs, len), TKA_MAX_SPLITS, &p.own_splits, &p.own_tps);
   return p;
 }
 
@@ -194,12 +203,13 @@ Plan plan_decode(const tka_kvq_flash_decode_args* a) {
 // L2 and the memory-side cache: the blocks of a head run side by side) and conversions, fewer start and end sooner and leave the
 // CU to more workgroups, so the rule goes by the size of the products, query rows x heads x positions.  Times by sixteens 1 / 2 / 4 /
 // 8 / 16 in us, suffixes of 100:
-//   16 x 8 x 4 (64 rows), 1000 positions    16 bit  0.5 M   10.7 / 11.0 / 16.3 / 13.4 / 13.9
+//   16 x 8 x 4 (64 rows), 1000 positions    16 bit  0.5 M   10.6 / 10.9 / 16.2 / 13.4 / 13.9
 //   10 x 8 x 4 (40), 8192                   int8    2.6 M   16.8 / 17.5 / 19.5 / 20.3 / 21.3
-//   16 x 8 x 4, 8192                        16 bit  4.2 M   23.2 / 21.1 / 24.0 / 27.0 / 26.5
-//   32 x 8 x 4 (128), 8192                  16 bit  8.4 M   33.8 / 26.1 / 27.3 / 35.6 / 31.6
-//   16 x 8 x 4, 32768                       16 bit   17 M   66.6 / 47.4 / 41.4 / 55.5 / 59.1
+//   16 x 8 x 4, 8192                        16 bit  4.2 M   20.8 / 18.7 / 24.0 / 27.0 / 26.5
+//   32 x 8 x 4 (128), 8192                  16 bit  8.4 M   30.4 / 23.4 / 27.4 / 35.6 / 31.6
+//   16 x 8 x 4, 32768                       16 bit   17 M   57.1 / 40.9 / 41.5 / 55.5 / 59.1
 //   32 x 8 x 4, 16384                       e4m3     17 M   38.6 / 30.0 / 32.8 / 34.9 / 33.9
+//   32 x 8 x 4, 32768                       16 bit   34 M   92.6 / 57.3 / 47.2 / 61.8 / 62.1
 //   64 x 8 x 8 (512), 8192                  e4m3     34 M      - / 49.2 / 52.6 / 47.2 / 43.8
 //   32 x 8 x 4, 65536                       int8     67 M      - / 84.2 / 81.1 / 73.5 / 76.9
 //   64 x 8 x 8, 32768                       16 bit  134 M      -  / 206 /  130 /  129 /  131
@@ -207,7 +217,7 @@ Plan plan_decode(const tka_kvq_flash_decode_args* a) {
 int prefix_row_tiles(int64_t query_rows, int64_t positions, bool wide16) {
   const int64_t work = query_rows * positions;
   if (query_rows <= 16 || work <= 5 << 19) return 1;
-  if (query_rows <= 32 || work <= (wide16 ? 9 << 20 : 28 << 20)) return 2;
+  if (query_rows <= 32 || work <= (wide16 ? 17 << 20 : 28 << 20)) return 2;
   if (wide16 || query_rows <= 64) return 4;   // (16-bit rows have no conversion to share: blocks of 128 and 256 do not win)
   return query_rows <= 128 ? 8 : 16;
 }
@@ -228,7 +238,9 @@ Plan plan_prefix(const tka_prefix_decode_args* a) {
     const bool wide16 = a->prefix.format == TKA_KV_16BIT;
     p.row_tiles = hook ? (wide16 ? std::min(hook, 4) : hook) : prefix_row_tiles(query_rows, heads * a->prefix.rows, wide16);
     p.row_blocks = (int)((query_rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-    cut(a->prefix.rows, a->num_splits ? a->num_splits : (p.row_tiles == 4 || p.row_tiles == 16 ? 256 : 512) / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
+    // One workgroup a CU for 16-bit rows and the blocks that fill a CU, two for 8-bit rows (16 x 8 x 4 over 8192 rows of 16 bits with 512
+    // workgroups 21.1 us, with 256 18.7; 32768 rows of e4m3 32.8 and 34.8, with 1024 41.1).
+    cut(a->prefix.rows, a->num_splits ? a->num_splits : (wide16 || p.row_tiles == 4 || p.row_tiles == 16 ? 256 : 512) / (heads * p.row_blocks), TKA_MAX_SPLITS / 2, &p.shared_splits, &p.shared_tps);
   }
   // The blocks of 256 query rows leave no room on a CU beside them (LDS), so that the suffixes would come after them, one workgroup
   // a CU.  Many short suffixes are attended to by the launch that joins the partials instead, three workgroups a CU: (batch x heads
