@@ -795,26 +795,29 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
   attend_own<DT, FMT, INDEXED, kWaves>(p, blockIdx.x - shared_items, sh, sh_ids);
 }
 
-// More query rows than a wave can hold: the waves of a workgroup take 32 query rows of a head each and go through the tokens
-// together, a macro tile of 32 tokens a wave at a time.  Each wave loads its 32 tokens, converts and transposes them into
-// matrix operands once and leaves those in LDS, from where all waves read them; the rows of the next macro tile are on
-// their way meanwhile.
+// More query rows than a wave can hold: the waves of a workgroup take 32 query rows of a head each and go through the tokens together,
+// a set of WAVES / 2 tiles at a time.  One half of the waves loads, converts and transposes the tiles of the even sets into matrix
+// operands and leaves those in LDS, the other half those of the odd sets, each one set ahead, so that of the two waves of a SIMD one
+// converts while the other multiplies and a set takes one barrier; all waves read all operands (8 KB of keys and 8 of values a tile).
+// 64 x 8 x 8 query rows over 32768 + 256 rows of e4m3: 96 us in both launches, 720 TFLOP/s of products (with all waves converting
+// a tile of eight at a time, and two barriers, 106).  What bounds it is the issue of a SIMD: in 92 us before that step its matrix
+// unit was busy for 34 % of the cycles and its vector unit for 44 %, with waves waiting a third of their time for operands or barriers.
 template <int DT, int FMT, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAttendParams p) {
   static_assert(kQuantised<FMT>, "");
   using State = Rows<DT, FMT, 2>;
-  constexpr int kMacro = WAVES * kTile;
+  constexpr int kSet = WAVES / 2;   // tiles of a set
   // Value operands with their scales in them, over a power of two of the tile: exact in e4m3, where scales are powers of two
   // (but for what lies 2^-24 below the tile's largest), and off by half a step of fp16 twice in int8, which is left to the
   // weights where these are kept in two parts.  It saves a product for every weight.
   constexpr bool kScaled = FMT == TKA_KV_E4M3 || !State::kSplit;
   struct Operands {
-    u32x4 frag[WAVES][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
-    float ks[WAVES][kTile], vs[WAVES][kTile];
-    float tile_scale[WAVES];
+    u32x4 frag[kSet][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
+    float ks[kSet][kTile], vs[kSet][kTile];
+    float tile_scale[kSet];
   };
   __shared__ union {
-    Operands of;
+    Operands sets[2];
     AttendLds join;
   } sh;
   const uint32_t shared_items = (uint32_t)(p.row_blocks * p.num_kv_heads * p.shared_splits);
@@ -848,8 +851,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       scale = (lane < kTile ? it.ks : it.vs)[(int64_t)(start + min(lane & (kTile - 1), dense.last)) * it.scale_n];
     }
   };
+  const int half = wave / kSet, place = wave % kSet;   // this wave converts tile `place` of every other set
   // the operands of the tile in the registers, from position `tile` on
-  const auto stage = [&](int tile) {
+  const auto stage = [&](int tile, Operands& of) {
     const int token = lane & (kTile - 1);
     const bool cut = it.end - tile < kTile;
     const int start = tile_start(tile, it.end);
@@ -863,20 +867,20 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       top = power_above(__shfl(top, kWave - 1, kWave));
       _Float16 f = (_Float16)(scale * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, top)));
       if (cut && (start + token < tile || start + token >= it.end)) f = (_Float16)0.0f;
-      _Float16* held = (_Float16*)sh.of.vs[wave];
+      _Float16* held = (_Float16*)of.vs[place];
       if (lane >= kTile) held[token] = f;
-      if (lane == 0) sh.of.tile_scale[wave] = top;
+      if (lane == 0) of.tile_scale[place] = top;
       const u32x2 lo = *(const u32x2*)(held + 4 * j), hi = *(const u32x2*)(held + 16 + 4 * j);
       factor = (u32x4){lo[0], lo[1], hi[0], hi[1]};
-      if (lane < kTile) sh.of.ks[wave][token] = scale * p.scale_log2e;
+      if (lane < kTile) of.ks[place][token] = scale * p.scale_log2e;
     } else {
-      (lane < kTile ? sh.of.ks : sh.of.vs)[wave][token] = lane < kTile ? scale * p.scale_log2e : scale;
+      (lane < kTile ? of.ks : of.vs)[place][token] = lane < kTile ? scale * p.scale_log2e : scale;
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
-        sh.of.frag[wave][4 * x + kb][lane] = k_frag<FMT, State::kQF16>(kt[x], kb);
+        of.frag[place][4 * x + kb][lane] = k_frag<FMT, State::kQF16>(kt[x], kb);
         __builtin_amdgcn_sched_barrier(0);   // (one operand after the other: all at once they do not fit the registers)
       }
     const auto values = [&](auto d) {
@@ -890,8 +894,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
           odd[w] = as_bits(as_f16(odd[w]) * as_f16(factor[w]));
         }
       }
-      sh.of.frag[wave][8 + 2 * D][lane] = even;
-      sh.of.frag[wave][9 + 2 * D][lane] = odd;
+      of.frag[place][8 + 2 * D][lane] = even;
+      of.frag[place][9 + 2 * D][lane] = odd;
       __builtin_amdgcn_sched_barrier(0);
     };
     values(std::integral_constant<int, 0>());
@@ -900,36 +904,49 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
     values(std::integral_constant<int, 3>());
   };
 
-  load(it.begin + wave * kTile);
-  for (int macro = it.begin, rest = it.end - it.begin; rest > 0; macro += kMacro, rest -= kMacro) {
-    const int mine = macro + wave * kTile;
-    __syncthreads();   // (the operands of the last macro tile are done with)
-    if (wave * kTile < rest) stage(mine);
-    __syncthreads();
-    if (rest > kMacro) load(mine + kMacro);
+  const auto first_of = [&](int set) { return it.begin + (set * kSet + place) * kTile; };
+  const int tiles = (it.end - it.begin + kTile - 1) / kTile, num_sets = (tiles + kSet - 1) / kSet;
+  load(first_of(half));
+  if (half == 0) {
+    if (first_of(0) < it.end) stage(first_of(0), sh.sets[0]);
+    load(first_of(2));
+  }
+  __syncthreads();
+  for (int set = 0; set < num_sets; ++set, __syncthreads()) {
+    if (((set + 1) & 1) == half && set + 1 < num_sets) {
+      __builtin_amdgcn_s_setprio(1);   // (the others wait for it at the end of the set: 97.0 -> 96.2 us)
+      if (first_of(set + 1) < it.end) stage(first_of(set + 1), sh.sets[(set + 1) & 1]);
+      __builtin_amdgcn_s_setprio(0);
+      load(first_of(set + 3));
+    }
     if (idle) continue;
-    const int tiles = min((rest + kTile - 1) / kTile, WAVES);
-    for (int t = 0; t < tiles; ++t) {
-      const int tile = macro + t * kTile;
-      const bool cut = rest - t * kTile < kTile;
+    const Operands& of = sh.sets[set & 1];
+    const int count = min(tiles - set * kSet, kSet);
+    u32x4 vfr[8];
+    for (int t = 0; t < count; ++t) {
+      const int tile = it.begin + (set * kSet + t) * kTile;
+      const bool cut = it.end - tile < kTile;
       f32x4 sc[2][2];
-      rows.scores(sc, [&](int x, int kb) { return sh.of.frag[t][4 * x + kb][lane]; });
+      rows.scores(sc, [&](int x, int kb) { return of.frag[t][4 * x + kb][lane]; });
       float kf[8], vf[8], tile_scale = 0.0f;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const f32x4 a = *(const f32x4*)&sh.of.ks[t][16 * x + 4 * j], b = kScaled ? a : *(const f32x4*)&sh.of.vs[t][16 * x + 4 * j];
+        const f32x4 a = *(const f32x4*)&of.ks[t][16 * x + 4 * j], b = kScaled ? a : *(const f32x4*)&of.vs[t][16 * x + 4 * j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           kf[4 * x + i] = a[i];
           vf[4 * x + i] = b[i];
         }
       }
-      if constexpr (kScaled) tile_scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.of.tile_scale[t])));
+      if constexpr (kScaled) tile_scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, of.tile_scale[t])));
+#pragma unroll
+      for (int x = 0; x < 8; ++x) vfr[x] = of.frag[t][8 + x][lane];   // (on their way during the softmax: 99 -> 97 us)
+      __builtin_amdgcn_sched_barrier(0);
       rows.template attend<kScaled>(sc, kf, vf, tile_scale, cut ? tile_mask(tile_start(tile, it.end), tile, it.end) : 0u, cut,
                                     [&](auto d, u32x4* even, u32x4* odd) {
                                       constexpr int D = decltype(d)::value;
-                                      *even = sh.of.frag[t][8 + 2 * D][lane];
-                                      *odd = sh.of.frag[t][9 + 2 * D][lane];
+                                      *even = vfr[2 * D];
+                                      *odd = vfr[2 * D + 1];
                                     });
     }
   }
