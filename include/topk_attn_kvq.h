@@ -74,8 +74,8 @@ typedef struct tka_kvq_write_args {
 int tka_kvq_write(const tka_kvq_write_args* args);
 
 /* Row (b, start[b] + t, h) of the cache goes to row (b,t,h) of the outputs for t < count[b], as code * scale (fp32)
- * rounded to `dtype`, numbers beyond its range as its largest.  Output rows without a source (behind count[b], or from outside [0, rows)) keep what they hold; output rows
- * must be disjoint like those of a written cache. */
+ * rounded to `dtype`, numbers beyond its range as its largest.  Output rows without a source (behind count[b], or from
+ * outside [0, rows)) keep what they hold; output rows must be disjoint like those of a written cache. */
 typedef struct tka_kvq_read_args {
   tka_kv_cache cache;
   void* k;                /* device; rows as in tka_kvq_write_args                              */
@@ -110,7 +110,8 @@ int tka_kvq_scores(const tka_kvq_scores_args* args);
 
 /* out = softmax(scale * q.K^T) V over the rows t < kv_len[b], or over the listed rows.  A query without a row gets zeros
  * and lse = -infinity.  The entries of a list count as often as they stand in it; ids outside [0, kv_len[b]) are
- * skipped. */
+ * skipped.  Value scales are held relative to the largest one that was met: beside it, what rows of much smaller scales lose
+ * is below 2^-22 of the largest |value|. */
 typedef struct tka_kvq_flash_decode_args {
   tka_kv_cache cache;     /* stride_b = 0: shared by the batch                                  */
   const void* q;          /* device [batch][num_kv_heads*group][128]                            */
@@ -138,7 +139,7 @@ int tka_kvq_flash_decode(const tka_kvq_flash_decode_args* args);
 /* out[b] = softmax(scale * q[b].K^T) V over the rows of the prefix followed by the first suffix_len[b] rows of suffix
  * entry b: the prefix is read once for the whole batch.  Both caches have one format; `prefix.batch` is 1, `suffix.batch`
  * is the batch.  A prefix without rows (prefix.rows = 0) is allowed (its pointers are then not read), and so is a suffix
- * without rows (suffix.rows = 0, suffix.batch still the batch). */
+ * without rows (suffix.rows = 0, suffix.batch still the batch).  Value scales as in tka_kvq_flash_decode. */
 typedef struct tka_prefix_decode_args {
   tka_kv_cache prefix;
   tka_kv_cache suffix;

@@ -25,7 +25,16 @@
 // Results of waves and splits are joined normalised, out = sum (l_s 2^(m_s - M) / L) o_s: they stay in the range of V.
 //
 // A workgroup is one (source, batch entry or block of query rows, head, split); its waves take 32-token tiles in turn and
-// are joined in LDS, the splits by a second launch.  The shared source multiplies a block of 16 * RT query rows (entries x group) with each K / V tile.
+// are joined in LDS, the splits by a second launch.  The shared source multiplies a block of query rows (entries x group) with each
+// K / V tile.
+//
+// What bounds it: the bytes of the cache for a decode (4 x 8 x 32768 rows of e4m3, lengths from half of it to all, 225 MB: 44 us,
+// 5.1 TB/s); two launches of about 4 us each for a short call; the gather for a list (8 x 8 x 2128 of 32768 rows of int8: 15.3 us,
+// 11.7 of them in the first launch); the bytes, then the issue of the products, for a prefix (16 x 8 x 4 query rows over 32768 + 500
+// rows of 16 bits, 160 MB: 41 us, 3.9 TB/s; larger blocks of query rows: at kv_attend_wide_kernel).
+//
+// Joining the splits in the launch itself, by the last workgroup of a row, took longer than the second launch does (8 splits of one
+// head 8.7 us against 8.1, 32 heads 29.7 against 11.5: the XCDs have no L2 in common, so that flags and partials go through memory).
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -773,7 +782,8 @@ __device__ __forceinline__ void attend_own(const KvAttendParams& p, uint32_t own
   attend<DT, FMT, 1, INDEXED, WAVES>(p, item, sh, sh_ids);
 }
 
-// RT: sixteens of query rows that a workgroup of the shared source takes (0: there is no shared source)
+// RT: sixteens of query rows that a workgroup of the shared source takes (0: there is no shared source).  Each wave holds all of them and
+// has its tiles to itself: nothing is exchanged before the join.  RT = 4 takes the registers of a whole SIMD, RT = 2 those of a half.
 template <int DT, int FMT, int RT, bool INDEXED>
 __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_attend_kernel(KvAttendParams p) {
   __shared__ AttendLds sh;
@@ -800,8 +810,8 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
 // operands and leaves those in LDS, the other half those of the odd sets, each one set ahead, so that of the two waves of a SIMD one
 // converts while the other multiplies and a set takes one barrier; all waves read all operands (8 KB of keys and 8 of values a tile).
 // 64 x 8 x 8 query rows over 32768 + 256 rows of e4m3: 96 us in both launches, 720 TFLOP/s of products (with all waves converting
-// a tile of eight at a time, and two barriers, 106).  What bounds it is the issue of a SIMD: in 92 us before that step its matrix
-// unit was busy for 34 % of the cycles and its vector unit for 44 %, with waves waiting a third of their time for operands or barriers.
+// eight tiles at a time, and two barriers, 106).  What bounds it is the issue: its matrix units are busy 36 % of the 87 us and its
+// vector units half of them; a wave issues, waits to issue, and waits for operands or a barrier a third of its time each.
 template <int DT, int FMT, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAttendParams p) {
   static_assert(kQuantised<FMT>, "");
@@ -967,7 +977,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
 }
 
 // Short calls: one workgroup of eight waves per (entry, head) attends to everything and writes the result, one launch.  The
-// shared rows are then read for each entry.
+// shared rows are then read for each entry.  Bound by the launch: one sequence, 8 heads, 256 rows 6.3 us (split and joined 7.8).
 constexpr int kSoloWaves = 8;
 template <int DT, int FMT, bool SHARED, bool INDEXED>
 __global__ __launch_bounds__(kSoloWaves * kWave, 2) void kv_attend_solo_kernel(KvAttendParams p) {
@@ -1006,7 +1016,8 @@ __global__ __launch_bounds__(kThreads, 3) void kv_attend_join_kernel(KvAttendPar
   attend<DT, FMT, 1, false, kWaves, true>(p, item, sh, nullptr);
 }
 
-// One workgroup per query row: 32 lanes hold the 128 dims, eight groups of them take every eighth split.  A row whose sum is
+// The join of the splits, bound by the launch and by the partials (516 bytes each): 2.4 us for 8 rows of 8 splits, 4.2 us for 512 rows of
+// 16 to 34.  One workgroup per query row: 32 lanes hold the 128 dims, eight groups of them take every eighth split.  A row whose sum is
 // NaN stays NaN (an empty split holds zeros, so nothing has to be skipped); one without any key gets zeros and -infinity.
 constexpr int kCombineGroups = kThreads / 32;
 __global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttendParams p) {

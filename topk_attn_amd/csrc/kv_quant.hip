@@ -4,7 +4,10 @@
 //   kvq_read_kernel     code * scale, rounded to 16 bits
 //   kvq_scores_kernel   the canonical 16-part dot product of topk_attn.h with codes as keys, times the row's scale
 //
-// All three are bound by the bytes they move: 256 + 132 per row and direction, 132 per scored row.
+// All three are bound by the bytes they move: 256 + 132 per row and direction, 132 + 4 per scored row; short calls by the launch (3.8 to
+// 4.3 us from call to call).  Measured: 3 prompts of up to 16385 tokens, 8 heads, fp16 to int8, 254 MB: 49 us, 5.2 TB/s; 2 x 32768 tokens
+// back from int8 to bf16, 356 MB: 63 to 72 us, 5.0 to 5.7 TB/s; scores of 4 x 8 x 131072 rows of e4m3, 467 MB at lengths from half
+// of it to all: 74 us, 6.3 TB/s.  (A copy of 4 GiB reads and writes 4.6 TB/s here, a kernel that only reads 7.1.)
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -64,7 +67,8 @@ struct Codes<TKA_KV_INT8> {
   }
 };
 
-// Row of this lane group and the lane's place in it.  Tokens go fastest: 2^tile_log2 of them (32 on long calls) lie next
+// A row is eight lanes: its maximum stays in three DPP steps, a wave stores eight rows of codes of one head, 1 KB without gaps where the
+// cache lies head by head.  Row of this lane group and the lane's place in it.  Tokens go fastest: 2^tile_log2 of them (32 on long calls) lie next
 // to each other in the scales of a head, a whole line of them.
 struct CopyItem {
   bool there;

@@ -67,7 +67,7 @@ struct KvAttendParams {
   KvRows shared;
   int shared_splits;        // 0: no shared rows
   int shared_tps;           // tokens per split, a multiple of kAttendTile
-  int row_blocks;           // query rows of a head (batch * group) in blocks of 16 * RT
+  int row_blocks;           // query rows of a head (batch * group) in blocks of 16 * row_tiles
   KvRows own;
   int own_splits;           // 0: no own rows
   int own_tps;
@@ -86,7 +86,8 @@ struct KvAttendParams {
   float scale_log2e;
 };
 constexpr int kAttendTile = 32;   // tokens of a wave's tile
-// row_tiles: RT of the shared source; 0 = the short form, one workgroup per (entry, head) and one split of each source.
+// row_tiles: sixteens of query rows that a workgroup takes with each tile of the shared source: 1, 2, 4, in 8 bits also 8 and 16;
+// 0 = the short form, one workgroup per (entry, head) and one split of each source.
 int launch_kv_attend(const KvAttendParams& p, int dtype, int format, int row_tiles, hipStream_t stream);
 
 // The own rows (one workgroup per entry and head, whatever own_splits says) joined with num_splits partials of the shared ones.
