@@ -351,7 +351,8 @@ def test_every_block_size_where_it_can_go_wrong(row_tiles):
     test_many_short_suffixes_in_a_graph()
 
 
-@pytest.mark.parametrize("fmt,B,G,P", [("16bit", 3, 8, 40000), ("16bit", 40, 8, 60000), ("e4m3", 6, 8, 60000), ("int8", 40, 4, 200000), ("e4m3", 64, 8, 60000)])
+@pytest.mark.parametrize("fmt,B,G,P", [("16bit", 3, 8, 40000), ("16bit", 40, 8, 60000), ("e4m3", 6, 8, 60000), ("int8", 40, 4, 200000), ("e4m3", 64, 8, 60000),
+                                       ("e4m3", 32, 4, 380000)])
 def test_the_blocks_that_long_prefixes_choose(fmt, B, G, P):
     """Sizes at which the call itself takes blocks of 32, 64, 128 and 256 query rows; the output of a few entries is checked."""
     announce("prefix long %s B%d G%d P%d" % (fmt, B, G, P))

@@ -210,14 +210,15 @@ Plan plan_decode(const tka_kvq_flash_decode_args* a) {
 //   16 x 8 x 4, 32768                       16 bit   17 M   57.1 / 40.9 / 41.5 / 55.5 / 59.1
 //   32 x 8 x 4, 16384                       e4m3     17 M   38.6 / 30.0 / 32.8 / 34.9 / 33.9
 //   32 x 8 x 4, 32768                       16 bit   34 M   92.6 / 57.3 / 47.2 / 61.8 / 62.1
-//   64 x 8 x 8 (512), 8192                  e4m3     34 M      - / 49.2 / 52.6 / 47.2 / 43.8
-//   32 x 8 x 4, 65536                       int8     67 M      - / 84.2 / 81.1 / 73.5 / 76.9
+//   32 x 8 x 4, 32768                       e4m3     34 M      - / 44.8 / 47.0 / 48.1 / 46.2
+//   64 x 8 x 8 (512), 8192                  e4m3     34 M      - / 49.5 / 53.0 / 50.0 / 44.5
+//   20 x 8 x 4 (80), 100000                 int8     64 M      -  / 101 /  119 / 91.3 / 96.3
 //   64 x 8 x 8, 32768                       16 bit  134 M      -  / 206 /  130 /  129 /  131
-//   64 x 8 x 8, 32768                       e4m3    134 M      -  / 133 /  135 /  107 /  105
+//   64 x 8 x 8, 32768                       e4m3    134 M      -  / 133 /  135 /  107 / 97.0
 int prefix_row_tiles(int64_t query_rows, int64_t positions, bool wide16) {
   const int64_t work = query_rows * positions;
   if (query_rows <= 16 || work <= 5 << 19) return 1;
-  if (query_rows <= 32 || work <= (wide16 ? 17 << 20 : 28 << 20)) return 2;
+  if (query_rows <= 32 || work <= (wide16 ? 17 << 20 : query_rows <= 128 ? 44 << 20 : 28 << 20)) return 2;
   if (wide16 || query_rows <= 64) return 4;   // (16-bit rows have no conversion to share: blocks of 128 and 256 do not win)
   return query_rows <= 128 ? 8 : 16;
 }
