@@ -212,7 +212,7 @@ def test_launches_stay_within_the_limit():
         a.prefix.rows, a.suffix.rows, a.suffix.batch, a.group = rows, 0, 32768, 1
         a.prefix.num_kv_heads = a.suffix.num_kv_heads = 256
         a.q_stride_b = a.out_stride_b = 256 * 128
-        assert lib.tka_prefix_decode(C.byref(a)) == (UNSUPPORTED if rows == 200 else L.TKA_EWORKSPACE)
+        assert lib.tka_prefix_decode(C.byref(a)) == L.TKA_EWORKSPACE      # (blocks of query rows: fewer workgroups)
         a.suffix.batch, a.group = 32768, 4
         a.q_stride_b = a.out_stride_b = 1024 * 128
         assert lib.tka_prefix_decode(C.byref(a)) == UNSUPPORTED

@@ -173,7 +173,7 @@ struct Plan {
   bool to_workspace() const { return parts() > 1 || join_own; }
 };
 
-// Calls of up to this many positions per (entry, head) take one launch of one workgroup each instead of a split and a join
+// Decodes of up to this many positions per (entry, head) take one launch of one workgroup each instead of a split and a join
 // (one sequence, 8 heads, group 4: 6.4 against 7.9 us at 256 positions, 8.6 against 7.8 at 512; host-bound below).
 constexpr int64_t kSoloLen = 256;
 
@@ -223,20 +223,29 @@ int prefix_row_tiles(int64_t query_rows, int64_t positions, bool wide16) {
   return query_rows <= 128 ? 8 : 16;
 }
 
+// Short calls: one workgroup per (entry, head) attends to prefix and suffix and writes the result; the prefix is then read, and widened,
+// for each entry.  Against the split form, us: 4 x 2 x 4 over 250 + 50 rows of 16 bits 7.0 and 7.7 (400 + 50: 8.6 and 7.7), 16 x 8 x 4 over
+// 250 + 50 7.3 and 8.4, 64 x 16 x 4 over 250 + 20 23.5 and 17.2; 8 bits: 32 x 8 x 4 over 250 + 20 7.5 and 10.1, 64 x 8 x 8 over 400 + 100
+// 16.7 and 19.6, but 4 x 8 x 4 over 400 + 50 8.3 and 7.9.
+bool prefix_in_one(int64_t segs, int64_t len, bool wide16) {
+  if (wide16) return segs <= 256 && len <= 320;
+  return len <= 320 || (segs >= 192 && len <= 512);
+}
+
 std::atomic<int> g_row_tiles{0};   // tka_kvq_test_row_tiles
 
 Plan plan_prefix(const tka_prefix_decode_args* a) {
   Plan p = {1, 0, 0, 0, 0, 0, false};
   const int64_t heads = a->prefix.num_kv_heads, batch = a->suffix.batch, query_rows = batch * a->group;
   const int hook = g_row_tiles.load(std::memory_order_relaxed);
-  if (!a->num_splits && !hook && a->prefix.rows + a->suffix.rows <= kSoloLen) {
+  const bool wide16 = a->prefix.format == TKA_KV_16BIT;
+  if (!a->num_splits && !hook && prefix_in_one(heads * batch, a->prefix.rows + a->suffix.rows, wide16)) {
     p.row_tiles = 0;
     if (a->prefix.rows) cut(a->prefix.rows, 1, 1, &p.shared_splits, &p.shared_tps);
     if (a->suffix.rows) cut(a->suffix.rows, 1, 1, &p.own_splits, &p.own_tps);
     return p;
   }
   if (a->prefix.rows) {
-    const bool wide16 = a->prefix.format == TKA_KV_16BIT;
     p.row_tiles = hook ? (wide16 ? std::min(hook, 4) : hook) : prefix_row_tiles(query_rows, heads * a->prefix.rows, wide16);
     p.row_blocks = (int)((query_rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     // One workgroup a CU for 16-bit rows and the blocks that fill a CU, two for 8-bit rows (16 x 8 x 4 over 8192 rows of 16 bits with 512
