@@ -809,7 +809,7 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
 // a set of WAVES / 2 tiles at a time.  One half of the waves loads, converts and transposes the tiles of the even sets into matrix
 // operands and leaves those in LDS, the other half those of the odd sets, each one set ahead, so that of the two waves of a SIMD one
 // converts while the other multiplies and a set takes one barrier; all waves read all operands (8 KB of keys and 8 of values a tile).
-// 64 x 8 x 8 query rows over 32768 + 256 rows of e4m3: 96 us in both launches, 720 TFLOP/s of products (with all waves converting
+// 64 x 8 x 8 query rows over 32768 + 256 rows of e4m3: 97 us in both launches, 715 TFLOP/s of products (with all waves converting
 // eight tiles at a time, and two barriers, 106).  What bounds it is the issue: its matrix units are busy 36 % of the 87 us and its
 // vector units half of them; a wave issues, waits to issue, and waits for operands or a barrier a third of its time each.
 template <int DT, int FMT, int WAVES>
