@@ -223,6 +223,12 @@ __device__ __forceinline__ float power_above(float x) {
   return __builtin_bit_cast(float, min(max(e, 17u << 23), 0x7e000000u));
 }
 
+// The power of two at or above |x|, 2^-126 at least and 2^125 at most.
+__device__ __forceinline__ float power_at(float x) {
+  const uint32_t e = (min(__builtin_bit_cast(uint32_t, x) & 0x7fffffffu, 0x7e000000u) + 0x7fffffu) & 0x7f800000u;
+  return __builtin_bit_cast(float, max(e, 1u << 23));
+}
+
 // What a wave holds of its 16 RT query rows (row n of each sixteen in the lanes n, n + 16, n + 32, n + 48).
 template <int DT, int FMT, int RT>
 struct Rows {
@@ -285,10 +291,10 @@ struct Rows {
   // The rest of it.  kf: factors of the slot tokens' logits, vs: their value scales; masked: bit s = slot s has no row
   // (any_masked: some lane has one); value_frags(D, even, odd): operands of output dims 2 D and 2 D + 1.
   // tile_scale (SCALED): a power of two that the value operands have been divided by, with their scales in them (vs is then not
-  // looked at).
+  // looked at); rest, where `uneven`: what the tile's scales have beside that, for the weights.
   template <bool SCALED, typename ValueFrags>
-  __device__ __forceinline__ void attend(f32x4 (&sc)[RT][2], float (&kf)[8], float (&vs)[8], float tile_scale, uint32_t masked, bool any_masked,
-                                         ValueFrags value_frags) {
+  __device__ __forceinline__ void attend(f32x4 (&sc)[RT][2], float (&kf)[8], float (&vs)[8], float tile_scale, bool uneven, const float* rest,
+                                         uint32_t masked, bool any_masked, ValueFrags value_frags) {
     // masked slots have no weight (and their value rows are zeros: no 0 * inf, no 0 * NaN)
     if (any_masked) {
 #pragma unroll
@@ -349,8 +355,20 @@ struct Rows {
       }
     }
 #pragma unroll
+    for (int r = 0; r < RT; ++r) l_run[r] = SCALED ? __builtin_fmaf(sum[r], back, l_run[r]) : l_run[r] + sum[r];
+    if (SCALED && uneven) {
+      const float* of = rest + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const f32x4 f = *(const f32x4*)(of + 16 * x);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ps[r][4 * x + i] *= f[i];
+      }
+    }
+#pragma unroll
     for (int r = 0; r < RT; ++r) {
-      l_run[r] = SCALED ? __builtin_fmaf(sum[r], back, l_run[r]) : l_run[r] + sum[r];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float a = ps[r][2 * w], b = ps[r][2 * w + 1];
@@ -622,7 +640,7 @@ __device__ __forceinline__ void attend(const KvAttendParams& p, const AttendItem
         rows.scores(sc, [&](int x, int kb) { return k_frag<FMT, Rows<DT, FMT, RT>::kQF16>(kt[x], kb); });
         if (more) load_keys(next);
         if (any_masked) clear_masked<FMT>(masked, vr);
-        rows.template attend<false>(sc, kf, vs, 0.0f, masked, any_masked, [&](auto d, u32x4* even, u32x4* odd) { v_frags<FMT, decltype(d)::value>(vr, even, odd); });
+        rows.template attend<false>(sc, kf, vs, 0.0f, false, nullptr, masked, any_masked, [&](auto d, u32x4* even, u32x4* odd) { v_frags<FMT, decltype(d)::value>(vr, even, odd); });
         if (!more) break;
         load_values(next);
         tile = next_tile;
@@ -817,14 +835,18 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
   static_assert(kQuantised<FMT>, "");
   using State = Rows<DT, FMT, 2>;
   constexpr int kSet = WAVES / 2;   // tiles of a set
-  // Value operands with their scales in them, over a power of two of the tile: exact in e4m3, where scales are powers of two
-  // (but for what lies 2^-24 below the tile's largest), and off by half a step of fp16 twice in int8, which is left to the
-  // weights where these are kept in two parts.  It saves a product for every weight.
-  constexpr bool kScaled = FMT == TKA_KV_E4M3 || !State::kSplit;
+  // Value operands with their scales in them, over a power of two of the tile, which saves a product for every weight.  e4m3: of
+  // a scale only the power of two at or above it, so that the operands are exact (but for what lies 2^-24 below the tile's
+  // largest); the rest of it, in (1/2, 1], goes to the weights in fp32 in the tiles where it is not 1 throughout (it is 1
+  // for what tka_kvq_write makes).  int8, whose scales are hardly ever powers of two, with bf16 queries: the whole scale, off by
+  // half a step of fp16 twice (2^-10 of a value, below the 2^-8 of a bf16 output).  int8 with fp16 queries: the weights, which
+  // are then kept in two parts, take the scales.
+  constexpr bool kPowers = FMT == TKA_KV_E4M3, kScaled = kPowers || !State::kSplit;
   struct Operands {
     u32x4 frag[kSet][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
     float ks[kSet][kTile], vs[kSet][kTile];
-    float tile_scale[kSet];
+    float rest[kPowers ? kSet : 1][kTile];
+    f32x2 tile_scale[kSet];        // and whether `rest` has anything but ones
   };
   __shared__ union {
     Operands sets[2];
@@ -875,11 +897,21 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
 #pragma unroll
       for (int x = 1; x < kTile; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
       top = power_above(__shfl(top, kWave - 1, kWave));
-      _Float16 f = (_Float16)(scale * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, top)));
-      if (cut && (start + token < tile || start + token >= it.end)) f = (_Float16)0.0f;
+      const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, top));   // 1 / top
+      const bool there = !cut || (start + token >= tile && start + token < it.end);
+      _Float16 f = (_Float16)(scale * unit);
+      bool uneven = false;
+      if constexpr (kPowers) {
+        const float power = power_at(scale);
+        const float rest = there ? __builtin_ldexpf(fabsf(scale), 127 - (int)(__builtin_bit_cast(uint32_t, power) >> 23)) : 1.0f;
+        f = (_Float16)(__builtin_copysignf(power, scale) * unit);
+        uneven = __ballot(lane >= kTile && rest != 1.0f) != 0ull;
+        if (lane >= kTile) of.rest[place][token] = rest;
+      }
+      if (!there) f = (_Float16)0.0f;
       _Float16* held = (_Float16*)of.vs[place];
       if (lane >= kTile) held[token] = f;
-      if (lane == 0) of.tile_scale[place] = top;
+      if (lane == 0) of.tile_scale[place] = (f32x2){top, uneven ? 1.0f : 0.0f};
       const u32x2 lo = *(const u32x2*)(held + 4 * j), hi = *(const u32x2*)(held + 16 + 4 * j);
       factor = (u32x4){lo[0], lo[1], hi[0], hi[1]};
       if (lane < kTile) of.ks[place][token] = scale * p.scale_log2e;
@@ -939,6 +971,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       f32x4 sc[2][2];
       rows.scores(sc, [&](int x, int kb) { return of.frag[t][4 * x + kb][lane]; });
       float kf[8], vf[8], tile_scale = 0.0f;
+      bool uneven = false;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const f32x4 a = *(const f32x4*)&of.ks[t][16 * x + 4 * j], b = kScaled ? a : *(const f32x4*)&of.vs[t][16 * x + 4 * j];
@@ -948,11 +981,16 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
           vf[4 * x + i] = b[i];
         }
       }
-      if constexpr (kScaled) tile_scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, of.tile_scale[t])));
+      if constexpr (kScaled) {
+        const f32x2 held = of.tile_scale[t];
+        const float top = held[0], flag = held[1];
+        tile_scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
+        if constexpr (kPowers) uneven = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, flag)) != 0;
+      }
 #pragma unroll
       for (int x = 0; x < 8; ++x) vfr[x] = of.frag[t][8 + x][lane];   // (on their way during the softmax: 99 -> 97 us)
       __builtin_amdgcn_sched_barrier(0);
-      rows.template attend<kScaled>(sc, kf, vf, tile_scale, cut ? tile_mask(tile_start(tile, it.end), tile, it.end) : 0u, cut,
+      rows.template attend<kScaled>(sc, kf, vf, tile_scale, uneven, of.rest[kPowers ? t : 0], cut ? tile_mask(tile_start(tile, it.end), tile, it.end) : 0u, cut,
                                     [&](auto d, u32x4* even, u32x4* odd) {
                                       constexpr int D = decltype(d)::value;
                                       *even = vfr[2 * D];
