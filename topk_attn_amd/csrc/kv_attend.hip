@@ -12,7 +12,7 @@
 //
 // 8-bit rows: a code is exact as a 16-bit number, so K codes go to the type of q and V codes to fp16; the scale of a key
 // row multiplies its logits, that of a value row its weight, both in fp32.  Weights enter the second product as fp16:
-// 2^(x - m) * (scale / cap) * 2^9, with cap a power of two no scale seen so far exceeds (accumulators move with it) and m a
+// 2^(x - m) * (scale / cap) * 2^9, with cap a power of two no scale seen so far exceeds (up to 2^127; accumulators move with it) and m a
 // reference that no logit x exceeds by more than 6: at most 2^15, rounded by 2^-11 of themselves down to 2^-14 and by 2^-25
 // below.  Where q is fp16 the remainder goes through the matrix cores as a second operand, so that the weights are as
 // exact as the output.  16-bit rows: fp16 weights are held the same way without a cap; bf16 weights have fp32's range but
@@ -185,7 +185,8 @@ struct AttendLds {
 template <bool F16>
 constexpr float kWeightLog2 = F16 ? 9.0f : -32.0f;   // weights are held times 2^this
 template <bool F16>
-constexpr float kMostWeight = F16 ? 32768.0f : 0x1p-26f;   // 2^6 times that: the reference moves when eight weights add up to more
+constexpr float kMostWeight = F16 ? 32704.0f : 0x1p-26f;   // 2^6 times that: the reference moves when eight weights add up to more
+// (in fp16 a little less: a weight times a scale of just below twice the largest cap, 2^127, has to stay below 65504)
 
 // Positions [begin, end) of the rows of one entry and head (of a token list where there is one).
 struct AttendSource {
@@ -217,15 +218,19 @@ __device__ __forceinline__ void store_row(const KvAttendParams& p, int b, int hq
     p.out_lse[(((int64_t)b * p.num_kv_heads) << p.group_log2) + hq] = L > 0.0f || L != L ? (M + (__builtin_log2f(L) - l_log2)) * 0.69314718055994531f : -INFINITY;
 }
 
-// Twice the power of two at or above x (x >= 0), 2^-110 at least.
+// Twice the power of two at or above x (x >= 0), 2^-110 at least and 2^127 at most.
 __device__ __forceinline__ float power_above(float x) {
   const uint32_t e = ((__builtin_bit_cast(uint32_t, x) + 0x7fffffu) & 0x7f800000u) + 0x800000u;
-  return __builtin_bit_cast(float, min(max(e, 17u << 23), 0x7e000000u));
+  return __builtin_bit_cast(float, min(max(e, 17u << 23), 0x7f000000u));
+}
+// 1 / x of a power of two from 2^-126 to 2^127 (whose reciprocal is a subnormal number).
+__device__ __forceinline__ float power_inverse(float x) {
+  return __builtin_bit_cast(float, max((254u << 23) - __builtin_bit_cast(uint32_t, x), 0x400000u));
 }
 
-// The power of two at or above |x|, 2^-126 at least and 2^125 at most.
+// The power of two at or above |x|, 2^-126 at least and 2^127 at most.
 __device__ __forceinline__ float power_at(float x) {
-  const uint32_t e = (min(__builtin_bit_cast(uint32_t, x) & 0x7fffffffu, 0x7e000000u) + 0x7fffffu) & 0x7f800000u;
+  const uint32_t e = (min(__builtin_bit_cast(uint32_t, x) & 0x7fffffffu, 0x7f000000u) + 0x7fffffu) & 0x7f800000u;
   return __builtin_bit_cast(float, max(e, 1u << 23));
 }
 
@@ -318,7 +323,7 @@ struct Rows {
 #pragma unroll
       for (int s = 1; s < 8; ++s) top = fmaxf(top, fabsf(vs[s]));
       if (__ballot(top > cap) != 0ull) raise_cap(power_above(max_over_quarters(top)));
-      const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, cap));   // 1 / cap
+      const float unit = power_inverse(cap);
 #pragma unroll
       for (int s = 0; s < 8; ++s) weight[s] = vs[s] * unit;
     }
@@ -837,7 +842,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
   constexpr int kSet = WAVES / 2;   // tiles of a set
   // Value operands with their scales in them, over a power of two of the tile, which saves a product for every weight.  e4m3: of
   // a scale only the power of two at or above it, so that the operands are exact (but for what lies 2^-24 below the tile's
-  // largest); the rest of it, in (1/2, 1], goes to the weights in fp32 in the tiles where it is not 1 throughout (it is 1
+  // largest); the rest of it, in (1/2, 1] (below 2 for scales beyond 2^127), goes to the weights in fp32 in the tiles where it is not 1 throughout (it is 1
   // for what tka_kvq_write makes).  int8, whose scales are hardly ever powers of two, with bf16 queries: the whole scale, off by
   // half a step of fp16 twice (2^-10 of a value, below the 2^-8 of a bf16 output).  int8 with fp16 queries: the weights, which
   // are then kept in two parts, take the scales.
@@ -897,7 +902,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
 #pragma unroll
       for (int x = 1; x < kTile; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
       top = power_above(__shfl(top, kWave - 1, kWave));
-      const float unit = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, top));   // 1 / top
+      const float unit = power_inverse(top);
       const bool there = !cut || (start + token >= tile && start + token < it.end);
       _Float16 f = (_Float16)(scale * unit);
       bool uneven = false;
