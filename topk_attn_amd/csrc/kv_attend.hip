@@ -228,6 +228,14 @@ __device__ __forceinline__ float power_inverse(float x) {
   return __builtin_bit_cast(float, max((254u << 23) - __builtin_bit_cast(uint32_t, x), 0x400000u));
 }
 
+// What lanes of the wave have stored to LDS is there for its other lanes to load (the LDS serves a wave's accesses in order: this
+// holds the compiler to that order, and costs nothing).
+__device__ __forceinline__ void wave_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The power of two at or above |x|, 2^-126 at least and 2^127 at most.
 __device__ __forceinline__ float power_at(float x) {
   const uint32_t e = (min(__builtin_bit_cast(uint32_t, x) & 0x7fffffffu, 0x7f000000u) + 0x7fffffu) & 0x7f800000u;
@@ -917,6 +925,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
       _Float16* held = (_Float16*)of.vs[place];
       if (lane >= kTile) held[token] = f;
       if (lane == 0) of.tile_scale[place] = (f32x2){top, uneven ? 1.0f : 0.0f};
+      wave_exchange();
       const u32x2 lo = *(const u32x2*)(held + 4 * j), hi = *(const u32x2*)(held + 16 + 4 * j);
       factor = (u32x4){lo[0], lo[1], hi[0], hi[1]};
       if (lane < kTile) of.ks[place][token] = scale * p.scale_log2e;
