@@ -19,7 +19,8 @@
  *   TKA_KV_INT8   scale = max(fp32(A / 127), 2^-126);  code = x * min(fp32(127 / A), 2^126) in fp32, rounded to the
  *                 nearest whole number, ties to even (-127 .. 127).
  * A row that holds an infinity or a NaN gets scale = NaN and codes 0: it reads back as NaN and shows wherever it is used.
- * The readers accept any code byte and any fp32 scale: they need not come from tka_kvq_write.
+ * The readers accept any code byte and any fp32 scale: they need not come from tka_kvq_write.  (The attention multiplies a key
+ * row's scale by the call's scale * log2 e first: a product beyond fp32's range counts as infinite.)
  */
 #ifndef TOPK_ATTN_KVQ_H_
 #define TOPK_ATTN_KVQ_H_

@@ -29,9 +29,12 @@
 // K / V tile.
 //
 // What bounds it: the bytes of the cache for a decode (4 x 8 x 32768 rows of e4m3, lengths from half of it to all, 225 MB: 44 us,
-// 5.1 TB/s); two launches of about 4 us each for a short call; the gather for a list (8 x 8 x 2128 of 32768 rows of int8: 15.3 us,
-// 11.7 of them in the first launch); the bytes, then the issue of the products, for a prefix (16 x 8 x 4 query rows over 32768 + 500
-// rows of 16 bits, 160 MB: 41 us, 3.9 TB/s; larger blocks of query rows: at kv_attend_wide_kernel).
+// 5.1 TB/s); two launches of about 4 us each for a short call; the latency of the gather for a list (8 x 8 lists of up to 2128 of 32768
+// rows of int8, three quarters full: 15.3 us, 11.8 of them in the first launch, which fetches 39 MB of lines, 3.3 TB/s; 384 workgroups, some
+// of them without rows, are one or two waves a SIMD with three rounds of dependent loads each; e4m3 15.0); the bytes, then the issue of the products,
+// for a prefix (16 x 8 x 4 query rows over 32768 + 500 rows of 16 bits, 159 MB: 41 us, 3.9 TB/s; larger blocks of query rows: at
+// kv_attend_wide_kernel).  Splits are cut for the capacity of a cache, not for the lengths it holds: 4 x 8 heads that hold 16384 tokens
+// take 26.5 us in a cache of 16384 and 118 in one of 131072, where most workgroups have no rows (4096 tokens: 12.6 and 64).
 //
 // Joining the splits in the launch itself, by the last workgroup of a row, took longer than the second launch does (8 splits of one
 // head 8.7 us against 8.1, 32 heads 29.7 against 11.5: the XCDs have no L2 in common, so that flags and partials go through memory).
@@ -472,7 +475,11 @@ struct DenseTiles {
 #pragma unroll
       for (int y = 0; y < KTile<FMT>::kLoads; ++y) kt[x].w[y] = *(const u32x4*)(base + k_off[x] + 64 * y);
   }
-  // STREAM: rows that nobody else reads (a request covers whole lines; 4 x 8 x 32768 rows of 8 bits: 52.2 -> 47.7 us).
+  // STREAM: with the hint that the rows are not read again (a request covers whole lines).  All but the blocks of 128 and 256 query
+  // rows give it, also for rows that several workgroups read.  With and without it, us: decode of 4 x 8 x 32768 rows of e4m3 46.1 and 53.0;
+  // prefixes of 32768 rows of 16 bits, 16 x 8 x 4 39.8 and 45.8, 32 x 8 x 4 47.1 and 50.2, 64 x 8 x 8 134 and 141; one-launch calls the
+  // same; it loses for 8-bit rows that are shared: prefixes of e4m3, 16 x 8 x 4 32.3 and 29.8, 32 x 8 x 4 45.9 and 41.4, a decode of
+  // 16 x 8 x 4 over one cache of 32768 110 and 106.
   template <bool STREAM>
   __device__ __forceinline__ void value_rows(const AttendSource& it, int start, VRow<FMT> (&vr)[8]) const {
     const unsigned char* base = it.v + (int64_t)start * it.stride_n;
@@ -840,9 +847,10 @@ __global__ __launch_bounds__(kThreads, RT >= 4 ? 1 : (RT == 2 ? 2 : 3)) void kv_
 // a set of WAVES / 2 tiles at a time.  One half of the waves loads, converts and transposes the tiles of the even sets into matrix
 // operands and leaves those in LDS, the other half those of the odd sets, each one set ahead, so that of the two waves of a SIMD one
 // converts while the other multiplies and a set takes one barrier; all waves read all operands (8 KB of keys and 8 of values a tile).
-// 64 x 8 x 8 query rows over 32768 + 256 rows of e4m3: 97 us in both launches, 715 TFLOP/s of products (with all waves converting
-// eight tiles at a time, and two barriers, 106).  What bounds it is the issue: its matrix units are busy 36 % of the 87 us and its
-// vector units half of them; a wave issues, waits to issue, and waits for operands or a barrier a third of its time each.
+// 64 x 8 x 8 query rows over 32768 + 256 rows of e4m3, bf16: 97 to 99 us in both launches, 705 TFLOP/s of products (with all waves
+// converting eight tiles at a time, and two barriers, 106); int8 96; fp16, whose weights are in two parts: e4m3 116, int8 122.  What
+// bounds it is the issue: its matrix units are busy 36 % of the 88 us and its vector units half of them; a wave issues, waits to
+// issue, and waits for operands or a barrier a third of its time each.
 template <int DT, int FMT, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAttendParams p) {
   static_assert(kQuantised<FMT>, "");
@@ -850,8 +858,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
   constexpr int kSet = WAVES / 2;   // tiles of a set
   // Value operands with their scales in them, over a power of two of the tile, which saves a product for every weight.  e4m3: of
   // a scale only the power of two at or above it, so that the operands are exact (but for what lies 2^-24 below the tile's
-  // largest); the rest of it, in (1/2, 1] (below 2 for scales beyond 2^127), goes to the weights in fp32 in the tiles where it is not 1 throughout (it is 1
-  // for what tka_kvq_write makes).  int8, whose scales are hardly ever powers of two, with bf16 queries: the whole scale, off by
+  // largest); the rest of it, in (1/2, 1] (below 2 for scales beyond 2^127), goes to the weights in fp32 in the tiles where it is
+  // not 1 throughout (it is 1 for what tka_kvq_write makes; 64 x 8 x 8 over 32768 rows with other scales: fp16 115 -> 121 us, bf16 97 -> 99).  int8, whose scales are hardly ever powers of two, with bf16 queries: the whole scale, off by
   // half a step of fp16 twice (2^-10 of a value, below the 2^-8 of a bf16 output).  int8 with fp16 queries: the weights, which
   // are then kept in two parts, take the scales.
   constexpr bool kPowers = FMT == TKA_KV_E4M3, kScaled = kPowers || !State::kSplit;
