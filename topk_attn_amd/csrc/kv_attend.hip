@@ -859,9 +859,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_attend_wide_kernel(KvAtte
   // Value operands with their scales in them, over a power of two of the tile, which saves a product for every weight.  e4m3: of
   // a scale only the power of two at or above it, so that the operands are exact (but for what lies 2^-24 below the tile's
   // largest); the rest of it, in (1/2, 1] (below 2 for scales beyond 2^127), goes to the weights in fp32 in the tiles where it is
-  // not 1 throughout (it is 1 for what tka_kvq_write makes; 64 x 8 x 8 over 32768 rows with other scales: fp16 115 -> 121 us, bf16 97 -> 99).  int8, whose scales are hardly ever powers of two, with bf16 queries: the whole scale, off by
-  // half a step of fp16 twice (2^-10 of a value, below the 2^-8 of a bf16 output).  int8 with fp16 queries: the weights, which
-  // are then kept in two parts, take the scales.
+  // not 1 throughout (it is 1 for what tka_kvq_write makes; 64 x 8 x 8 over 32768 rows with other scales: fp16 115 -> 121 us,
+  // bf16 97 -> 99).  int8, whose scales are hardly ever powers of two, with bf16 queries: the whole scale, off by half a step of
+  // fp16 twice (2^-10 of a value, below the 2^-8 of a bf16 output).  int8 with fp16 queries: the weights, which are then kept in
+  // two parts, take the scales.
   constexpr bool kPowers = FMT == TKA_KV_E4M3, kScaled = kPowers || !State::kSplit;
   struct Operands {
     u32x4 frag[kSet][16][kWave];   // of a 32-token tile: K (x, kb) at 4 x + kb, V^T of dim c at 8 + c
